@@ -23,8 +23,20 @@ LINEAR_REUSE_WQ, LINEAR_REUSE_GQ = 32, 64
 LINEAR_OPERANDS_PACKED = 128
 LINEAR_SPLITK_WORKSPACE = 256
 LINEAR_FP32_ACCURACY = 512
+MASK_NONE, MASK_KEPT, MASK_ADD_F32, MASK_ADD_BF16 = 0, 1, 2, 3
 
 _i64, _int, _u32, _u64, _ptr = ctypes.c_int64, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, ctypes.c_void_p
+
+
+class AttnArgs(ctypes.Structure):
+    """``axs6_attn_args`` of include/axs6_b200.h, field by field."""
+    _fields_ = ([(n, _ptr) for n in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")]
+                + [(n + "_strides", _i64 * 3) for n in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")]
+                + [(n, _ptr) for n in ("row_max", "row_sum", "lse", "key_lengths", "mask")] + [("mask_strides", _i64 * 4)]
+                + [(n, _i64) for n in ("batch", "q_heads", "k_heads", "q_len", "k_len", "head_size", "window")]
+                + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("dtype", "causal", "mask_kind", "reserved")]
+                + [("workspace", _ptr), ("workspace_bytes", _i64)])
+
 
 # name -> (restype, argtypes); mirrors include/axs6_b200.h one to one
 SIGNATURES = {
@@ -59,6 +71,15 @@ SIGNATURES = {
     "axs6_linear_bwd": (_int, [_ptr, _int, _i64, _ptr, _ptr, _int, _i64, _ptr, _int, _i64, _ptr, _i64, _ptr,
                                _i64, _i64, _i64, _int, _int, _u32, _u64, _u64, _ptr, _ptr, _ptr, _ptr, _ptr, _ptr]),
     "axs6_transpose_f32": (_int, [_ptr, _ptr, _i64, _i64, _i64, _i64, _ptr]),
+    "axs6_rotary": (_int, [_ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _int, _i64, _i64, _i64, _i64,
+                           _ptr, _int, _i64, _i64, _ptr, ctypes.c_float, _int, _int, _ptr]),
+    "axs6_distill_fwd": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _int, _i64, _ptr, _i64, _i64, ctypes.c_float, _int,
+                                _ptr, _ptr, _ptr, _ptr]),
+    "axs6_distill_bwd": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _int, _i64, _ptr, _i64, _i64, ctypes.c_float,
+                                _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
+    "axs6_attn_fwd": (_int, [ctypes.POINTER(AttnArgs), _ptr]),
+    "axs6_attn_bwd": (_int, [ctypes.POINTER(AttnArgs), _ptr]),
+    "axs6_attn_workspace_bytes": (_i64, [ctypes.POINTER(AttnArgs), _int]),
 }
 
 _lib = None

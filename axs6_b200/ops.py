@@ -722,3 +722,248 @@ def transpose_f32(t: torch.Tensor) -> torch.Tensor:
                                             ld, _stream(t.device))
     _lib.check("axs6_transpose_f32", st)
     return out[:, :rows]
+
+
+# ------------------------------------------------------------------------------- rotary positions
+def _heads_view(t: torch.Tensor) -> torch.Tensor:
+    """(batch, heads, tokens, size) with adjacent values: the tensor itself, or a contiguous copy."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _strides3(t: torch.Tensor):
+    import ctypes
+    return (ctypes.c_int64 * 3)(*t.stride()[:3])
+
+
+def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor, gain: float = 1.0,
+           interleaved: bool = False, inverse: bool = False, who: str = "rotary"):
+    """Rotated copies of ``q`` and ``k`` (batch, heads, tokens, size; either may be None) in one launch.  ``turns``: int64 bits of
+    each pair's fraction of a turn per position; ``inverse`` turns the other way (the gradient)."""
+    given = [t for t in (q, k) if t is not None]
+    if not given:
+        raise ValueError(f"{who} needs q or k")
+    for t in given:
+        _check_input(t, who)
+        if t.dim() != 4:
+            raise ValueError(f"{who} takes tensors of (batch, heads, tokens, size), got {tuple(t.shape)}")
+        if t.dtype not in _DT:
+            raise TypeError(f"{who} takes fp32 or bf16 tensors, got {t.dtype}")
+    ref = given[0]
+    batch, _, tokens, size = ref.shape
+    if k is not None and q is not None and (k.shape[0], k.shape[2], k.shape[3]) != (batch, tokens, size):
+        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or size")
+    rotated = 2 * turns.numel()
+    if rotated > size:
+        raise ValueError(f"{who}: {rotated} values to rotate in heads of {size}")
+    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) not in ((tokens,), (batch, tokens)):
+        raise ValueError(f"{who}: positions must be int32 or int64 of shape ({tokens},) or ({batch}, {tokens}), got "
+                         f"{positions.dtype} {tuple(positions.shape)}")
+    if turns.dtype != torch.int64 or turns.dim() != 1:
+        raise ValueError(f"{who}: turns must be a 1-D int64 tensor")
+    if any(t.dtype != ref.dtype for t in given):
+        raise ValueError(f"{who}: q and k differ in type")
+    if any(t.device != ref.device for t in (*given, positions, turns)):
+        raise ValueError(f"{who}: tensors on different devices")
+    turns = turns.contiguous()
+    x = [None if t is None else _heads_view(t) for t in (q, k)]
+    y = [None if t is None else torch.empty_like(t) for t in x]
+    if any(t is not None and t.stride(-1) != 1 and t.shape[-1] > 1 for t in y):
+        y = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in x]
+
+    def side(a, b):
+        return (None, None, 0, None, None) if a is None else (a.data_ptr(), b.data_ptr(), a.shape[1], _strides3(a), _strides3(b))
+    pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
+    with _on(ref.device):
+        st = _lib.load().axs6_rotary(*side(x[0], y[0]), *side(x[1], y[1]), _DT[ref.dtype], batch, tokens, size, rotated,
+                                     positions.data_ptr(), int(positions.dtype == torch.int64), pb, pt, turns.data_ptr(),
+                                     float(gain), int(interleaved), int(inverse), _stream(ref.device))
+    _lib.check("axs6_rotary", st)
+    return y[0], y[1]
+
+
+# ------------------------------------------------------------------------------------ distillation
+def distill_fwd(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, temperature: float, reduction: int,
+                who: str = "axs_distillation_unified"):
+    """-> (loss, logits (rows, vocab), teacher (rows, k), index (rows, k), row statistics (rows, 2), count or None): what the
+    backward call takes.  ``reduction`` 0 none, 1 sum, 2 mean."""
+    for t in (logits, teacher, index):
+        _check_input(t, who)
+    if teacher.shape != index.shape or logits.shape[:-1] != index.shape[:-1]:
+        raise ValueError(f"{who}: logits {tuple(logits.shape)}, teacher_logits {tuple(teacher.shape)} and teacher_index "
+                         f"{tuple(index.shape)} do not belong together")
+    if index.dtype.is_floating_point or index.dtype.is_complex or index.dtype == torch.bool:
+        raise TypeError(f"{who}: teacher_index must be integers, got {index.dtype}")
+    if not logits.is_floating_point() or not teacher.is_floating_point():
+        raise TypeError(f"{who}: logits and teacher_logits must be floating point")
+    if not 1 <= index.shape[-1] <= 1024:
+        raise ValueError(f"{who}: between 1 and 1024 slots a position, got {index.shape[-1]}")
+    if logits.shape[-1] < 1:
+        raise ValueError(f"{who}: empty vocabulary")
+    if teacher.device != logits.device or index.device != logits.device:
+        raise ValueError(f"{who}: tensors on different devices")
+    z, rows, vocab, ldz = _as_rows(logits.detach())
+    t, _, slots, ldt = _as_rows(teacher.detach())
+    ix = index.reshape(-1, slots).to(torch.int64)
+    if ix.stride(1) != 1 and slots > 1:
+        ix = ix.contiguous()
+    dev = logits.device
+    row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    reduced = torch.empty(2, dtype=torch.float32, device=dev) if reduction else None
+    with _on(dev):
+        st = _lib.load().axs6_distill_fwd(z.data_ptr(), _DT[z.dtype], rows, vocab, ldz, t.data_ptr(), _DT[t.dtype], ldt, ix.data_ptr(),
+                                          ix.stride(0), slots, temperature, reduction, row_loss.data_ptr(), stats.data_ptr(),
+                                          reduced.data_ptr() if reduced is not None else None, _stream(dev))
+    _lib.check("axs6_distill_fwd", st)
+    loss = row_loss.reshape(logits.shape[:-1]) if reduced is None else reduced[0]
+    return loss, z, t, ix, stats, reduced[1:] if reduction == 2 else None
+
+
+def distill_bwd(z: torch.Tensor, t: torch.Tensor, ix: torch.Tensor, stats: torch.Tensor, upstream: torch.Tensor,
+                count: torch.Tensor | None, temperature: float) -> torch.Tensor:
+    """Gradient of the logits (rows, vocab) in their type; ``upstream``: one fp32 value, or one per row."""
+    rows, vocab = z.shape
+    up = upstream.to(torch.float32)
+    if up.dim():
+        up = up.reshape(-1)
+    grad = torch.empty((rows, vocab), dtype=z.dtype, device=z.device)
+    with _on(z.device):
+        st = _lib.load().axs6_distill_bwd(z.data_ptr(), _DT[z.dtype], rows, vocab, z.stride(0), t.data_ptr(), _DT[t.dtype], t.stride(0),
+                                          ix.data_ptr(), ix.stride(0), t.shape[1], temperature, stats.data_ptr(), up.data_ptr(),
+                                          up.stride(0) if up.dim() else 0, count.data_ptr() if count is not None else None,
+                                          grad.data_ptr(), vocab, _stream(z.device))
+    _lib.check("axs6_distill_bwd", st)
+    return grad
+
+
+# --------------------------------------------------------------------------------------- attention
+def _attn_operand(t: torch.Tensor) -> torch.Tensor:
+    """A tensor the kernels can read: values adjacent and, for bf16, 16-byte aligned rows and no overlapping ones; a padded
+    copy otherwise."""
+    if t.numel() == 0:
+        return t
+    if t.dtype == torch.float32:
+        return _heads_view(t)
+    ok = (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0
+    if ok and all(n == 1 or (s % 8 == 0 and s > 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
+        return t
+    size = t.shape[-1]
+    buf = torch.empty((*t.shape[:3], _r8(size)), dtype=t.dtype, device=t.device)[..., :size]
+    return buf.copy_(t)
+
+
+def _attn_strides(t: torch.Tensor):
+    """Strides {batch, head, token}; those of extents of one, which mean nothing, as if the tensor were packed."""
+    s = list(t.stride()[:3])
+    pitch = _r8(t.shape[3])
+    for d in (2, 1, 0):
+        if t.shape[d] == 1:
+            s[d] = pitch
+        pitch = max(pitch, s[d] * t.shape[d])
+    return s
+
+
+def _attn_args(tensors: dict, stats, lse, key_lengths, mask, scale: float, causal: bool, window: int) -> "_lib.AttnArgs":
+    a = _lib.AttnArgs()
+    for name, t in tensors.items():
+        setattr(a, name, t.data_ptr())
+        getattr(a, name + "_strides")[:] = _attn_strides(t)
+    q, k = tensors["q"], tensors["k"]
+    a.row_max, a.row_sum = stats[0].data_ptr(), stats[1].data_ptr()
+    a.lse = lse.data_ptr() if lse is not None else None
+    a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
+    if mask is not None:
+        a.mask = mask.data_ptr()
+        a.mask_strides[:] = mask.stride()
+        a.mask_kind = {torch.bool: _lib.MASK_KEPT, torch.float32: _lib.MASK_ADD_F32, torch.bfloat16: _lib.MASK_ADD_BF16}[mask.dtype]
+    a.batch, a.q_heads, a.q_len, a.head_size = q.shape
+    a.k_heads, a.k_len = k.shape[1:3]
+    a.window, a.scale, a.dtype, a.causal = window, scale, _DT[q.dtype], int(causal)
+    return a
+
+
+def _attn_workspace(a, backward: int, dev):
+    import ctypes
+    n = int(_lib.load().axs6_attn_workspace_bytes(ctypes.byref(a), backward))
+    if not n:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), n
+    return ws
+
+
+def attention_check(q, k, v, key_lengths, mask, scale, causal, window, who: str):
+    """Checks the arguments of an attention call -> (mask expanded to (batch, heads, queries, keys) or None, scale, window)."""
+    for t in (q, k, v):
+        _check_input(t, who)
+        if t.dim() != 4:
+            raise ValueError(f"{who} takes tensors of (batch, heads, tokens, size), got {tuple(t.shape)}")
+        if t.dtype not in _DT:
+            raise TypeError(f"{who} takes fp32 or bf16 tensors, got {t.dtype}")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise TypeError(f"{who}: q, k and v differ in type")
+    batch, heads, q_len, size = q.shape
+    if k.shape != v.shape or k.shape[0] != batch or k.shape[3] != size:
+        raise ValueError(f"{who}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not belong together")
+    if (heads % k.shape[1] if k.shape[1] else heads) != 0:
+        raise ValueError(f"{who}: {heads} query heads over {k.shape[1]} key heads")
+    if not 1 <= size <= 128:
+        raise ValueError(f"{who}: heads of 1 to 128 values, got {size}")
+    scale = size ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"{who}: scale must be positive and finite, got {scale}")
+    if window is not None and (not causal or int(window) < 1):
+        raise ValueError(f"{who}: window must be at least 1 and goes with causal=True")
+    if key_lengths is not None and (key_lengths.dtype != torch.int32 or tuple(key_lengths.shape) != (batch,)):
+        raise ValueError(f"{who}: key_lengths must be int32 of shape ({batch},)")
+    if mask is not None:
+        if mask.dtype not in (torch.bool, torch.float32, torch.bfloat16):
+            raise TypeError(f"{who}: mask must be bool, fp32 or bf16, got {mask.dtype}")
+        if mask.requires_grad:
+            raise ValueError(f"{who}: no gradient is computed for the mask")
+        mask = mask.expand(batch, heads, q_len, k.shape[2])
+    if any(t is not None and t.device != q.device for t in (k, v, key_lengths, mask)):
+        raise ValueError(f"{who}: tensors on different devices")
+    return mask, scale, 0 if window is None else int(window)
+
+
+def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window: int, want_lse: bool):
+    """-> (o shaped and laid out like q, row statistics (2, batch, heads, queries), lse or None, the operands as read)."""
+    import ctypes
+    q, k, v = (_attn_operand(t) for t in (q, k, v))
+    dev = q.device
+    o = torch.empty_like(q)
+    if o.numel() and _attn_operand(o) is not o:
+        o = torch.empty((*q.shape[:3], _r8(q.shape[3])), dtype=q.dtype, device=dev)[..., :q.shape[3]]
+    stats = torch.empty((2, *q.shape[:3]), dtype=torch.float32, device=dev)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
+    key_lengths = key_lengths.contiguous() if key_lengths is not None else None
+    a = _attn_args({"q": q, "k": k, "v": v, "o": o}, stats, lse, key_lengths, mask, scale, causal, window)
+    with _on(dev):
+        ws = _attn_workspace(a, 0, dev)
+        st = _lib.load().axs6_attn_fwd(ctypes.byref(a), _stream(dev))
+    _lib.check("axs6_attn_fwd", st)
+    del ws
+    return o, stats, lse, q, k, v
+
+
+def attention_bwd(d_o, q, k, v, o, stats, key_lengths, mask, scale: float, causal: bool, window: int):
+    """-> (dq, dk, dv), each laid out like the tensor it belongs to."""
+    import ctypes
+    dev = q.device
+    d_o = _attn_operand(d_o)
+    grads = []
+    for t in (q, k, v):
+        g = torch.empty_like(t)
+        if g.numel() and _attn_operand(g) is not g:
+            g = torch.empty((*t.shape[:3], _r8(t.shape[3])), dtype=t.dtype, device=dev)[..., :t.shape[3]]
+        grads.append(g)
+    key_lengths = key_lengths.contiguous() if key_lengths is not None else None
+    a = _attn_args({"q": q, "k": k, "v": v, "o": o, "d_o": d_o, "dq": grads[0], "dk": grads[1], "dv": grads[2]}, stats, None,
+                   key_lengths, mask, scale, causal, window)
+    with _on(dev):
+        ws = _attn_workspace(a, 1, dev)
+        st = _lib.load().axs6_attn_bwd(ctypes.byref(a), _stream(dev))
+    _lib.check("axs6_attn_bwd", st)
+    del ws
+    return tuple(grads)

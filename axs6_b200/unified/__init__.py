@@ -7,6 +7,9 @@ from .distributed import AXS6GradCompressor, axs6_gradient_hook, axs6_gradient_h
 from .quantize_unified import quantization_error_unified
 from .triton_kernels import has_triton, triton_fused_fake_quantize, triton_fused_linear
 from .functional_unified import axs_linear_unified, axs_matmul_unified, fake_quantize_unified
+from .attention_unified import axs_attention_unified
+from .distillation_unified import AXSDistillationLoss, axs_distillation_unified
+from .rotary_unified import RotaryFrequencies, axs_rotary_unified, rotary_frequencies
 from .mixed_precision import (AXSLinearMixedPrecision, axs_linear_mixed_precision, convert_to_axs_mixed_precision,
                               estimate_memory_savings)
 from .modules_unified import (AXSEmbeddingUnified, AXSLayerNormUnified, AXSLinearUnified, AXSMultiheadAttentionUnified,
@@ -21,4 +24,5 @@ __all__ = ["fused_fake_quantize", "quantize_unified", "dequantize_unified", "NF5
            "AXSLayerNormUnified", "AXSEmbeddingUnified", "AXSMultiheadAttentionUnified", "AmaxEMA",
            "AXSTrainingPipelineUnified", "quantization_error_unified", "BackendType", "clear_int8_weight_cache",
            "detect_best_backend", "has_triton", "triton_fused_fake_quantize", "triton_fused_linear", "AXS6GradCompressor",
-           "axs6_gradient_hook", "axs6_gradient_hook_packed"]
+           "axs6_gradient_hook", "axs6_gradient_hook_packed", "axs_attention_unified", "axs_distillation_unified", "AXSDistillationLoss",
+           "axs_rotary_unified", "rotary_frequencies", "RotaryFrequencies"]

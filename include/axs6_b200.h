@@ -380,6 +380,73 @@ int axs6_bias_grad_static(const void *g, int g_dtype, int64_t ldg, int64_t rows,
  * AXS6_LINEAR_SPLITK_WORKSPACE (0 when the product would not be split further). */
 int64_t axs6_linear_workspace_bytes(int what, int64_t M, int64_t N, int64_t K);
 
+/* ---- Operators of a decoder's training step beside the Linear (no counterparts in the reference, whose models use torch's attention,
+ * learned positions and cross entropy). */
+
+/* Rotary positions of the query heads and, in the same launch, the key heads: value pairs (a, b) become
+ * gain * (a cos t - b sin t, a sin t + b cos t), t = 2 pi * position * turns[pair] / 2^64, computed modulo a full turn in 64-bit
+ * fixed point; `inverse` negates t (the gradient).  The first `rotated` (even) values of a head are rotated, value i paired with
+ * i + rotated / 2, or 2 i with 2 i + 1 if `interleaved`; the others are copied.  Tensors are (batch, heads, tokens, head_size)
+ * with values adjacent and host arrays {batch, head, token} of strides in elements; q or k may have 0 heads (its pointers are then
+ * ignored).  `positions`: int64 if positions_64, else int32, any sign.  head_size <= 4096.  Outputs must not overlap inputs of another
+ * element (writing a tensor onto itself is fine).  Any alignment; 16-byte aligned pieces of both halves are moved whole. */
+int axs6_rotary(const void *q, void *q_out, int64_t q_heads, const int64_t *q_strides, const int64_t *q_out_strides,
+                const void *k, void *k_out, int64_t k_heads, const int64_t *k_strides, const int64_t *k_out_strides,
+                int dtype, int64_t batch, int64_t tokens, int64_t head_size, int64_t rotated,
+                const void *positions, int positions_64, int64_t pos_batch_stride, int64_t pos_token_stride,
+                const uint64_t *turns, float gain, int interleaved, int inverse, axs6_stream_t stream);
+
+/* Distillation from a teacher's top logits.  Row r: p = softmax(teacher / temperature) over the used slots, q = softmax(logits /
+ * temperature) over the vocabulary, row_loss = temperature^2 * sum p (log p - log q).  A slot is unused if its index lies outside
+ * [0, vocab) or its logit is -inf; a row without a used slot has loss 0 and is not counted.  1 <= slots <= 1024
+ * (AXS6_ERR_UNSUPPORTED above).  row_loss: rows floats, row_stats: 2 * rows floats for the backward call.  reduction 0: none,
+ * 1: reduced[0] = sum, 2: reduced[0] = mean over the counted rows; reduced[1] = their number, at least 1. */
+int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
+                     int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature, int reduction,
+                     float *row_loss, float *row_stats, float *reduced, axs6_stream_t stream);
+
+/* grad (rows, vocab), in the logits' type, = d (sum over rows of upstream[r * upstream_stride] * row_loss[r]) / d logits, divided by
+ * *count if that is not NULL (reduced[1] of a mean).  Slots that name the same index are added in slot order: no atomics. */
+int axs6_distill_bwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
+                     int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature,
+                     const float *row_stats, const float *upstream, int64_t upstream_stride, const float *count, void *grad,
+                     int64_t ld_grad, axs6_stream_t stream);
+
+enum { AXS6_MASK_NONE = 0, AXS6_MASK_KEPT = 1 /* one byte a pair, 0 hides it */, AXS6_MASK_ADD_F32 = 2, AXS6_MASK_ADD_BF16 = 3 /* added to
+       the scaled scores; -inf hides a pair */ };
+
+/* Tensors are (batch, heads, tokens, head_size) with values adjacent; strides {batch, head, token} in elements. */
+typedef struct axs6_attn_args {
+    const void *q, *k, *v;          /* q_heads a multiple of k_heads: query head h reads key head h / (q_heads / k_heads) */
+    void *o;                        /* written by the forward call, read by the backward call */
+    const void *d_o;                /* backward: gradient of o */
+    void *dq, *dk, *dv;             /* backward: written */
+    int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3], d_o_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
+    float *row_max, *row_sum;       /* (batch, q_heads, q_len): written by the forward, read by the backward call */
+    float *lse;                     /* NULL, or the same shape: log sum exp of a row's scores, -inf where it sees no key */
+    const int32_t *key_lengths;     /* NULL, or batch counts on the device: keys from there on are hidden, whatever they hold */
+    const void *mask;               /* mask_kind; strides {batch, head, query, key} in elements, 0 where it is shared */
+    int64_t mask_strides[4];
+    int64_t batch, q_heads, k_heads, q_len, k_len, head_size;
+    int64_t window;                 /* 0: none; with causal: a query sees the last `window` keys up to its own */
+    float scale;                    /* > 0 */
+    int32_t dtype, causal, mask_kind, reserved;
+    void *workspace;                /* axs6_attn_workspace_bytes(args, backward) bytes, 16-byte aligned (NULL if 0) */
+    int64_t workspace_bytes;
+} axs6_attn_args;
+
+/* o = softmax(scale q k^T + mask) v.  `causal`: query i stands at key i + k_len - q_len and sees no later key.  A row that sees no
+ * key gives zeros.  head_size <= 128 (AXS6_ERR_UNSUPPORTED above).  bf16 tensors: 16-byte aligned, strides multiples of 8 elements and not
+ * 0 where the extent is above 1 (AXS6_ERR_ALIGN otherwise); fp32 tensors: any. */
+int axs6_attn_fwd(const axs6_attn_args *args, axs6_stream_t stream);
+
+/* dq, dk, dv from d_o, recomputing the probabilities from row_max and row_sum.  Every output element has one writer and a fixed order
+ * of summation (shared key heads included): results are reproducible bit for bit. */
+int axs6_attn_bwd(const axs6_attn_args *args, axs6_stream_t stream);
+
+/* Bytes of `workspace` for a call with these sizes and type on the current device. */
+int64_t axs6_attn_workspace_bytes(const axs6_attn_args *args, int backward);
+
 #ifdef __cplusplus
 }
 #endif
