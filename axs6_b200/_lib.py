@@ -79,6 +79,7 @@ SIGNATURES = {
                                 _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
     "axs6_attn_fwd": (_int, [ctypes.POINTER(AttnArgs), _ptr]),
     "axs6_attn_bwd": (_int, [ctypes.POINTER(AttnArgs), _ptr]),
+    "axs6_attn_status": (_int, []),
     "axs6_attn_workspace_bytes": (_i64, [ctypes.POINTER(AttnArgs), _int]),
 }
 

@@ -6,7 +6,7 @@
 namespace axs6 {
 namespace attn {
 
-int fwd_bf16_simt(const Params &p, cudaStream_t st);
+int fwd_bf16(const Params &p, cudaStream_t st);
 int bwd_bf16_simt(const Params &p, cudaStream_t st);
 
 static int64_t rows_of(const axs6_attn_args &a) { return a.batch * a.q_heads * a.q_len; }
@@ -75,7 +75,7 @@ AXS6_API int axs6_attn_fwd(const axs6_attn_args *args, axs6_stream_t stream)
     const DeviceInfo &d = device_info();
     if (!d.valid || !d.ok) return AXS6_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return args->dtype == AXS6_F32 ? attn::fwd_fp32(p, st) : attn::fwd_bf16_simt(p, st);
+    return args->dtype == AXS6_F32 ? attn::fwd_fp32(p, st) : attn::fwd_bf16(p, st);
 }
 
 AXS6_API int axs6_attn_bwd(const axs6_attn_args *args, axs6_stream_t stream)

@@ -1,0 +1,180 @@
+// Tensor-core plumbing of the attention kernels: bounded barrier waits, tensor-memory access, tcgen05.mma with A in shared or in tensor
+// memory, and the shared-memory layout of (128 tokens x head) tiles.
+//
+// A tile is one or two boxes of 128 tokens x 64 values (128 bytes a row, 128-byte swizzle, 16 KB), the second for values 64..127.
+// The same bytes serve as a K-major operand (contraction over the head's values) and as an MN-major one (contraction over the
+// tokens): only the descriptors differ.
+#pragma once
+#include <cuda.h>
+
+#include "async_copy.cuh"
+#include "attn_common.cuh"
+
+namespace axs6 {
+namespace attn {
+namespace tc {
+
+using acp::smem_u32;
+
+constexpr int kRows = 128;                       // tokens of a tile
+constexpr uint32_t kBox = 128 * 128;             // bytes of a box
+constexpr uint32_t kWaitPolls = 1u << 20;        // of about a microsecond each, when a poll has to sleep
+
+static __device__ int g_status;                  // 0, or the code of the first wait that gave up (one translation unit includes this)
+
+// false: gave up, or somebody else did
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code, int *status)
+{
+    for (uint32_t i = 0; i < kWaitPolls; ++i) {
+        uint32_t ok;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+        if (ok) return true;
+        if ((i & 63u) == 63u && *(volatile int *)status != 0) return false;
+    }
+    atomicCAS(status, 0, code);
+    return false;
+}
+
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void commit(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+{
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// descriptor of a tile: version 1, 128-byte swizzle, 8-row groups 1024 bytes apart; lbo = distance of the 64-value boxes (MN-major only)
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo)
+{
+    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+// bf16 operands, fp32 result, M = 128
+__host__ __device__ constexpr uint32_t instr(int n, int b_mn)
+{
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+
+// D (128 x 128) = A B^T over the head's DP values, both tiles K-major
+template <int DP> __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
+{
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+        const uint32_t off = (uint32_t)(k / 4) * kBox + (uint32_t)(k % 4) * 32u;
+        mma_ss(d, desc(a + off, 0), desc(b + off, 0), instr(128, 0), k != 0);
+    }
+}
+// D (128 x DP) (+)= A B over 128 tokens: A is 128 x 128 bf16 in tensor memory (two values a column), B a tile, MN-major
+template <int DP> __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b, bool acc)
+{
+#pragma unroll
+    for (int k = 0; k < kRows / 16; ++k)
+        mma_ts(d, a + 8u * (uint32_t)k, desc(b + (uint32_t)k * 2048u, kBox), instr(DP, 1), acc || k != 0);
+}
+
+#define AXS6_REGS32(r) \
+    "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), \
+    "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),    \
+    "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),    \
+    "=r"(r[31])
+// 32 columns of this thread's lane
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,"
+                 "%24,%25,%26,%27,%28,%29,%30,%31}, [%32];" : AXS6_REGS32(r) : "r"(addr));
+}
+__device__ __forceinline__ void st32(uint32_t addr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,"
+                 "%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+                 "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
+                 "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi)
+{
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int row, int head, int b)
+{
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(row), "r"(head), "r"(b) : "memory");
+}
+// 128 tokens of one head; what lies outside the tensor arrives as zeros
+template <int DP> __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int row, int head, int b)
+{
+#pragma unroll
+    for (int c = 0; c < DP / 64; ++c) load_box(dst + (uint32_t)c * kBox, map, bar, c * 64, row, head, b);
+}
+// A whole warp: zeros into rows [row, 128) of a tile (0 * NaN would reach every row of a product over the tokens), seen by the tensor cores
+template <int DP> __device__ __forceinline__ void clear_rows(uint8_t *tile, int row)
+{
+    const int lane = threadIdx.x & 31;
+    for (int i = row * 8 + lane; i < kRows * 8; i += 32)
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) *reinterpret_cast<uint4 *>(tile + (size_t)c * kBox + (size_t)i * 16) = make_uint4(0u, 0u, 0u, 0u);
+    acp::fence_async_smem();
+    __syncwarp();
+}
+// One row of a result: 32 fp32 values from column `c0` on, scaled, rounded to bf16, in 16-byte pieces where the head is that long
+__device__ __forceinline__ void store_piece(__nv_bfloat16 *row, int c0, int d, const uint32_t *r, float f)
+{
+#pragma unroll
+    for (int e = 0; e < 32; e += 8) {
+        if (c0 + e + 8 <= d) {
+            uint4 w;
+            w.x = pack2(__uint_as_float(r[e]) * f, __uint_as_float(r[e + 1]) * f);
+            w.y = pack2(__uint_as_float(r[e + 2]) * f, __uint_as_float(r[e + 3]) * f);
+            w.z = pack2(__uint_as_float(r[e + 4]) * f, __uint_as_float(r[e + 5]) * f);
+            w.w = pack2(__uint_as_float(r[e + 6]) * f, __uint_as_float(r[e + 7]) * f);
+            *reinterpret_cast<uint4 *>(row + c0 + e) = w;
+        } else {
+            for (int x = e; x < e + 8; ++x)
+                if (c0 + x < d) row[c0 + x] = __float2bfloat16_rn(__uint_as_float(r[x]) * f);
+        }
+    }
+}
+
+// On the way out of a kernel in which a wait gave up: loads and products that were issued may still be running; they complete within
+// microseconds, so every thread lingers before shared and tensor memory are released.
+__device__ __forceinline__ void linger_if_failed(int *status)
+{
+    if (*(volatile int *)status != 0)
+        for (int i = 0; i < 200; ++i) __nanosleep(1000);
+}
+
+// ---------------------------------------------------------------------------------------------- host
+// (value, token, head, batch) map of a bf16 tensor, boxes of 64 x 128
+inline bool make_map(CUtensorMap *map, const void *ptr, int d, int64_t tokens, int64_t heads, int64_t batch, int64_t st, int64_t sh, int64_t sb)
+{
+    acp::EncodeTiledFn fn = acp::encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
+    const cuuint64_t any = (cuuint64_t)((d + 7) / 8 * 16);            // stride of an extent of one: never used, but checked
+    const cuuint64_t strides[3] = {tokens > 1 ? (cuuint64_t)st * 2 : any, heads > 1 ? (cuuint64_t)sh * 2 : any, batch > 1 ? (cuuint64_t)sb * 2 : any};
+    const cuuint32_t box[4] = {64, kRows, 1, 1}, es[4] = {1, 1, 1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace tc
+}  // namespace attn
+}  // namespace axs6
