@@ -32,7 +32,7 @@ class AttnArgs(ctypes.Structure):
     """``axs6_attn_args`` of include/axs6_b200.h, field by field."""
     _fields_ = ([(n, _ptr) for n in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")]
                 + [(n + "_strides", _i64 * 3) for n in ("q", "k", "v", "o", "d_o", "dq", "dk", "dv")]
-                + [(n, _ptr) for n in ("row_max", "row_sum", "lse", "key_lengths", "mask")] + [("mask_strides", _i64 * 4)]
+                + [(n, _ptr) for n in ("row_max", "row_sum", "lse", "o_low", "key_lengths", "mask")] + [("mask_strides", _i64 * 4)]
                 + [(n, _i64) for n in ("batch", "q_heads", "k_heads", "q_len", "k_len", "head_size", "window")]
                 + [("scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("dtype", "causal", "mask_kind", "reserved")]
                 + [("workspace", _ptr), ("workspace_bytes", _i64)])

@@ -7,7 +7,8 @@ namespace axs6 {
 namespace attn {
 
 int fwd_bf16(const Params &p, cudaStream_t st);
-int bwd_bf16_simt(const Params &p, cudaStream_t st);
+int bwd_bf16(const Params &p, cudaStream_t st);
+int64_t bwd_bf16_workspace(int64_t heads, int64_t q_len, bool mask);
 
 static int64_t rows_of(const axs6_attn_args &a) { return a.batch * a.q_heads * a.q_len; }
 
@@ -39,7 +40,7 @@ static int fill(Params &p, const axs6_attn_args &a, bool backward)
     p.dq = a.dq; p.dq_b = a.dq_strides[0]; p.dq_h = a.dq_strides[1]; p.dq_t = a.dq_strides[2];
     p.dk = a.dk; p.dk_b = a.dk_strides[0]; p.dk_h = a.dk_strides[1]; p.dk_t = a.dk_strides[2];
     p.dv = a.dv; p.dv_b = a.dv_strides[0]; p.dv_h = a.dv_strides[1]; p.dv_t = a.dv_strides[2];
-    p.row_max = a.row_max; p.row_sum = a.row_sum; p.lse = a.lse;
+    p.row_max = a.row_max; p.row_sum = a.row_sum; p.lse = a.lse; p.o_low = a.o_low;
     p.batch = (int)a.batch; p.q_heads = (int)a.q_heads; p.k_heads = (int)a.k_heads; p.group = a.k_heads ? (int)(a.q_heads / a.k_heads) : 1;
     p.q_len = (int)a.q_len; p.k_len = (int)a.k_len; p.head_size = (int)a.head_size; p.offset = p.k_len - p.q_len;
     p.causal = a.causal != 0; p.window = (int)(a.window < a.k_len ? a.window : a.k_len);      // a wider window hides nothing more
@@ -52,7 +53,8 @@ static int fill(Params &p, const axs6_attn_args &a, bool backward)
 
 static int64_t workspace(const axs6_attn_args &a, bool backward)
 {
-    return backward ? rows_of(a) * 4 : 0;                                // delta
+    if (!backward) return 0;
+    return a.dtype == AXS6_F32 ? rows_of(a) * 4 : bwd_bf16_workspace(a.batch * a.q_heads, a.q_len, a.mask_kind != AXS6_MASK_NONE);   // delta, ...
 }
 
 }  // namespace attn
@@ -93,5 +95,5 @@ AXS6_API int axs6_attn_bwd(const axs6_attn_args *args, axs6_stream_t stream)
     if (!d.valid || !d.ok) return AXS6_ERR_DEVICE;
     p.delta = static_cast<float *>(args->workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return args->dtype == AXS6_F32 ? attn::bwd_fp32(p, st) : attn::bwd_bf16_simt(p, st);
+    return args->dtype == AXS6_F32 ? attn::bwd_fp32(p, st) : attn::bwd_bf16(p, st);
 }

@@ -1,0 +1,510 @@
+// Attention backward on the tensor cores (bf16 tensors).  With c = scale log2 e and per row L = log2 of the forward's sum of exp2(c s):
+//     P = exp2(c S - L)    dV = P^T dO    dP = dO V^T    dS = P (dP - delta), delta = rowsum(dO O)    dQ = scale dS K    dK = scale dS^T Q
+// Two kernels, both recomputing S and dP: one per 128 keys (dK, dV; it also walks the query heads that share the key head), one per 128
+// queries (dQ).  That is 7 products a tile pair instead of the 5 that one kernel would need, and in return every output has one writer:
+// no fp32 copy of dQ in memory, no atomics, the same bits every time.  P and dS are rounded to bf16 as operands; everything else is fp32.
+//
+// Both kernels: warps 0-7 do the elementwise part (row = lane of tensor memory, warps 0-3 columns 0..63, warps 4-7 columns 64..127, 64 values
+// a thread), warp 8 issues the products, warp 9 loads.  P and dS go back to tensor memory over the columns they came from and are the
+// A operands of the next products, so shared memory holds nothing but loaded tiles.
+//
+// Bound: tensor cores, 4 (dK, dV) and 3 (dQ) products of 512 clocks a 128 x 128 tile at D = 128; exp2 takes 1024 clocks a tile in each.
+#pragma once
+#include "attn_tc.cuh"
+
+namespace axs6 {
+namespace attn {
+namespace tc {
+
+constexpr int kBwdThreads = 384;
+
+// Per row: what the probabilities are taken relative to, and delta; arrays padded to whole tiles per head, so that they load in bulk.
+// Rows behind the last query and rows without keys get L = +inf: probability 0.
+struct RowData {
+    float *shift;       // without a mask: L; with one: the row's maximum (its score may be the type's lowest value, where adding L is lost)
+    float *log_sum;     // with a mask: log2 of the row's sum
+    float *delta;
+    int padded;         // rows of a head
+};
+
+// 16 threads a row, 8 values each
+__global__ void __launch_bounds__(256) row_data_kernel(const Params p, const RowData w, int mask)
+{
+    const long long slots = (long long)p.batch * p.q_heads * w.padded;
+    const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
+    const int part = threadIdx.x & 15;
+    float s = 0.0f;
+    const int i = (int)(at % w.padded), bh = (int)(at / w.padded), h = bh % p.q_heads, b = bh / p.q_heads;
+    const bool real = at < slots && i < p.q_len;
+    if (real) {
+        const __nv_bfloat16 *o = static_cast<const __nv_bfloat16 *>(p.o.p) + b * p.o.b + h * p.o.h + i * p.o.t;
+        const __nv_bfloat16 *g = static_cast<const __nv_bfloat16 *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h + i * p.d_o.t;
+        const __nv_bfloat16 *low = p.o_low ? static_cast<const __nv_bfloat16 *>(p.o_low) + (o - static_cast<const __nv_bfloat16 *>(p.o.p)) : nullptr;
+        const int c = part * 8;
+        if (c + 8 <= p.head_size) {
+            const uint4 x = *reinterpret_cast<const uint4 *>(o + c), y = *reinterpret_cast<const uint4 *>(g + c);
+            const uint4 t = low ? *reinterpret_cast<const uint4 *>(low + c) : make_uint4(0u, 0u, 0u, 0u);
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, ts[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s = fmaf(__uint_as_float(xs[e] << 16) + __uint_as_float(ts[e] << 16), __uint_as_float(ys[e] << 16), s);
+                s = fmaf(__uint_as_float(xs[e] & 0xffff0000u) + __uint_as_float(ts[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), s);
+            }
+        } else {
+            for (int e = c; e < p.head_size; ++e) s = fmaf(__bfloat162float(o[e]) + (low ? __bfloat162float(low[e]) : 0.0f), __bfloat162float(g[e]), s);
+        }
+    }
+    for (int x = 8; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
+    if (part == 0 && at < slots) {
+        float shift = mask ? 0.0f : CUDART_INF_F, log_sum = CUDART_INF_F;
+        if (real) {
+            const long long src = (long long)bh * p.q_len + i;
+            const float m = p.row_max[src], l = p.row_sum[src];
+            if (l != 0.0f) { log_sum = log2f(l); shift = mask ? m : fmaf(m, kLog2e, log_sum); }
+        }
+        w.shift[at] = shift;
+        if (mask) w.log_sum[at] = log_sum;
+        w.delta[at] = s;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ dK, dV
+template <int DP> struct DkvSmem {
+    static constexpr uint32_t kTile = kBox * (DP / 64);
+    static constexpr int kStages = DP == 64 ? 4 : 2;
+    static constexpr uint32_t kVec = 3 * kRows * 4;                      // shift, log_sum, delta
+    static constexpr uint32_t kStage = 2 * kTile;                        // Q, dO
+    static constexpr uint32_t kRing = 2 * kTile, kVecs = kRing + kStages * kStage, kBars = kVecs + kStages * kVec;
+    static constexpr uint32_t kBytes = kBars + 256 + 1024;
+};
+
+template <int DP, bool kMask>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+           const __grid_constant__ CUtensorMap mg, const Params p, const RowData w)
+{
+    typedef DkvSmem<DP> L;
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t *gen = raw + (base - smem_u32(raw));
+    const uint32_t bars = base + L::kBars;
+    const uint32_t kv_full = bars, s_full = bars + 8, d_full = bars + 16, p_full = bars + 24, ds_full = bars + 32, done = bars + 40;
+    const auto q_full = [&](int s) { return bars + 48u + 8u * s; };
+    const auto g_full = [&](int s) { return bars + 48u + 8u * (L::kStages + s); };
+    const auto empty = [&](int s) { return bars + 48u + 8u * (2 * L::kStages + s); };
+    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + 48 + 24 * L::kStages);
+    int *status = &g_status;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = p.batch * p.k_heads;
+    const int bh = blockIdx.x % heads, kh = bh % p.k_heads, b = bh / p.k_heads;
+    const int j0 = (int)(blockIdx.x / heads) * kRows;                     // the first keys of a causal call have the longest walk: first
+    const int keys = keys_of(p, b);
+    const int j1 = j0 + kRows < keys ? j0 + kRows : keys;
+    const int ib = first_query(p, j0) / kRows;
+    const int ie = j0 < keys ? (end_query(p, j1) + kRows - 1) / kRows : 0;
+    const int per_head = ie > ib ? ie - ib : 0, steps = per_head * p.group;
+
+    if (threadIdx.x == 0) {
+        acp::mbar_init(kv_full, 1); acp::mbar_init(s_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(p_full, 256); acp::mbar_init(ds_full, 256);
+        acp::mbar_init(done, 1);
+        for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(q_full(s), 1); acp::mbar_init(g_full(s), 1); acp::mbar_init(empty(s), 1); }
+        acp::fence_barrier_init();
+        acp::fence_async_smem();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + 48u + 24u * L::kStages) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *slot;
+    const uint32_t tS = tmem, tD = tmem + 128u, tV = tmem + 256u, tK = tmem + 256u + DP;
+
+    if (warp == 9) {
+        if (lane == 0 && steps > 0) {
+            acp::mbar_expect_tx(kv_full, 2 * L::kTile);
+            load_tile<DP>(base, &mk, kv_full, j0, kh, b);
+            load_tile<DP>(base + L::kTile, &mv, kv_full, j0, kh, b);
+            int s = 0;
+            uint32_t ph = 0;
+            for (int x = 0; x < steps; ++x) {
+                if (!wait(empty(s), ph ^ 1u, 21, status)) break;
+                const int h = kh * p.group + x / per_head, i0 = (ib + x % per_head) * kRows;
+                const uint32_t dst = base + L::kRing + s * L::kStage, vec = base + L::kVecs + s * L::kVec;
+                const long long at = ((long long)b * p.q_heads + h) * w.padded + i0;
+                acp::mbar_expect_tx(q_full(s), L::kTile + (kMask ? 2 : 1) * kRows * 4);
+                load_tile<DP>(dst, &mq, q_full(s), i0, h, b);
+                acp::bulk_load(vec, w.shift + at, kRows * 4, q_full(s));
+                if (kMask) acp::bulk_load(vec + kRows * 4, w.log_sum + at, kRows * 4, q_full(s));
+                acp::mbar_expect_tx(g_full(s), L::kTile + kRows * 4);
+                load_tile<DP>(dst + L::kTile, &mg, g_full(s), i0, h, b);
+                acp::bulk_load(vec + 2 * kRows * 4, w.delta + at, kRows * 4, g_full(s));
+                if (++s == L::kStages) { s = 0; ph ^= 1u; }
+            }
+        }
+    } else if (warp == 8) {
+        if (lane == 0 && steps > 0) {
+            const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kStage; };
+            const auto phase = [&](int x) { return (uint32_t)(x / L::kStages) & 1u; };
+            bool ok = wait(kv_full, 0u, 22, status) && wait(q_full(0), 0u, 23, status);
+            if (ok) {
+                fence_after();
+                product_rows<DP>(tS, base, stage(0));                              // S^T = K Q^T
+                commit(s_full);
+                ok = wait(g_full(0), 0u, 24, status);
+            }
+            if (ok) {
+                fence_after();
+                product_rows<DP>(tD, base + L::kTile, stage(0) + L::kTile);        // dP^T = V dO^T
+                commit(d_full);
+            }
+            for (int x = 0; x < steps && ok; ++x) {
+                ok = wait(p_full, (uint32_t)x & 1u, 25, status);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(tV, tS, stage(x) + L::kTile, x != 0);           // dV += P^T dO
+                if (x + 1 < steps) {
+                    ok = wait(q_full((x + 1) % L::kStages), phase(x + 1), 26, status);
+                    if (!ok) break;
+                    fence_after();
+                    product_rows<DP>(tS, base, stage(x + 1));
+                    commit(s_full);
+                }
+                ok = wait(ds_full, (uint32_t)x & 1u, 27, status);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
+                commit(empty(x % L::kStages));
+                if (x + 1 < steps) {
+                    ok = wait(g_full((x + 1) % L::kStages), phase(x + 1), 28, status);
+                    if (!ok) break;
+                    fence_after();
+                    product_rows<DP>(tD, base + L::kTile, stage(x + 1) + L::kTile);
+                    commit(d_full);
+                }
+            }
+            if (ok) commit(done);
+        }
+    } else if (warp < 8) {
+        const int half = warp >> 2, row = threadIdx.x & 127, j = j0 + row;
+        const uint32_t mine = ((uint32_t)(warp & 3) << 21) + 64u * half;           // this warp's lanes and columns
+        const float c = p.scale * kLog2e;
+        bool ok = true;
+        for (int x = 0; x < steps; ++x) {
+            const int s = x % L::kStages, h = kh * p.group + x / per_head, i0 = (ib + x % per_head) * kRows;
+            const float *vec = reinterpret_cast<const float *>(gen + L::kVecs + s * L::kVec) + 64 * half;
+            ok = wait(s_full, (uint32_t)x & 1u, 29, status) && wait(q_full(s), (uint32_t)(x / L::kStages) & 1u, 30, status);
+            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            fence_after();
+            uint32_t r[64];
+            ld32(tS + mine, r);
+            ld32(tS + mine + 32u, r + 32);
+            wait_ld();
+            const int first = i0 + 64 * half;                                     // query of column 0 of this half
+            if (kMask) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) {
+                    const float y = sees(p, first + e, j, keys) ? masked_score(p, __uint_as_float(r[e]) * p.scale, b, h, first + e, j) : -CUDART_INF_F;
+                    r[e] = __float_as_uint(y == -CUDART_INF_F ? 0.0f : ex2(fmaf(y - vec[e], kLog2e, -vec[kRows + e])));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 64; e += 4) {
+                    const float4 sh = *reinterpret_cast<const float4 *>(vec + e);
+                    r[e] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e]), c, -sh.x)));
+                    r[e + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e + 1]), c, -sh.y)));
+                    r[e + 2] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e + 2]), c, -sh.z)));
+                    r[e + 3] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e + 3]), c, -sh.w)));
+                }
+                if ((p.causal && j0 + kRows - 1 > i0 + p.offset) || (p.window && j0 <= i0 + kRows - 1 + p.offset - p.window)) {
+                    // columns [lo, hi) see this key
+                    const int lo = p.causal ? j - p.offset - first : 0, hi = p.window ? j - p.offset + p.window - first : 64;
+#pragma unroll
+                    for (int e = 0; e < 64; ++e)
+                        if (e < lo || e >= hi) r[e] = 0u;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t y[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) y[z] = pack2(__uint_as_float(r[16 * e + 2 * z]), __uint_as_float(r[16 * e + 2 * z + 1]));
+                st8(tS + mine + 8u * e, y);
+            }
+            wait_st();
+            fence_before();
+            acp::mbar_arrive(p_full);
+            ok = wait(d_full, (uint32_t)x & 1u, 31, status) && wait(g_full(s), (uint32_t)(x / L::kStages) & 1u, 32, status);
+            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            fence_after();
+            uint32_t d[64];
+            ld32(tD + mine, d);
+            ld32(tD + mine + 32u, d + 32);
+            wait_ld();
+            const float *del = vec + 2 * kRows;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t y[8];
+#pragma unroll
+                for (int z = 0; z < 8; z += 2) {
+                    const int a = 16 * e + 2 * z;
+                    const float4 de = *reinterpret_cast<const float4 *>(del + a);
+                    y[z] = pack2(__uint_as_float(r[a]) * (__uint_as_float(d[a]) - de.x), __uint_as_float(r[a + 1]) * (__uint_as_float(d[a + 1]) - de.y));
+                    y[z + 1] = pack2(__uint_as_float(r[a + 2]) * (__uint_as_float(d[a + 2]) - de.z), __uint_as_float(r[a + 3]) * (__uint_as_float(d[a + 3]) - de.w));
+                }
+                st8(tD + mine + 8u * e, y);
+            }
+            wait_st();
+            fence_before();
+            acp::mbar_arrive(ds_full);
+        }
+        if (ok && steps > 0) {
+            ok = wait(done, 0u, 33, status);
+            ok = __all_sync(~0u, ok);
+            fence_after();
+        }
+        if (ok) {
+            // warps 0-3 write dV, warps 4-7 dK; keys behind the length get zeros
+            const uint32_t acc = (half ? tK : tV) + ((uint32_t)(warp & 3) << 21);
+            __nv_bfloat16 *out = half ? static_cast<__nv_bfloat16 *>(p.dk) + b * p.dk_b + kh * p.dk_h + j * p.dk_t
+                                      : static_cast<__nv_bfloat16 *>(p.dv) + b * p.dv_b + kh * p.dv_h + j * p.dv_t;
+            const float f = half ? p.scale : 1.0f;
+#pragma unroll 1
+            for (int x = 0; x < DP / 32; ++x) {
+                uint32_t o[32];
+                if (steps > 0) { ld32(acc + 32u * x, o); wait_ld(); }
+                if (steps == 0 || j >= keys) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (j < p.k_len) store_piece(out, 32 * x, p.head_size, o, f);
+            }
+        }
+    }
+    linger_if_failed(status);
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ dQ
+template <int DP> struct DqSmem {
+    static constexpr uint32_t kTile = kBox * (DP / 64);
+    static constexpr int kK = DP == 64 ? 4 : 3, kV = DP == 64 ? 4 : 2;
+    static constexpr uint32_t kRingK = 2 * kTile, kRingV = kRingK + kK * kTile, kBars = kRingV + kV * kTile;
+    static constexpr uint32_t kBytes = kBars + 256 + 1024;
+};
+
+template <int DP, bool kMask>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+          const __grid_constant__ CUtensorMap mg, const Params p, const RowData w)
+{
+    typedef DqSmem<DP> L;
+    extern __shared__ uint8_t raw[];
+    const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
+    uint8_t *gen = raw + (base - smem_u32(raw));
+    const uint32_t bars = base + L::kBars;
+    const uint32_t q_full = bars, g_full = bars + 8, d_full = bars + 16, ds_full = bars + 24, done = bars + 32, fix = bars + 40;
+    const auto s_full = [&](int x) { return bars + 48u + 8u * x; };
+    const auto k_full = [&](int s) { return bars + 64u + 8u * s; };
+    const auto k_empty = [&](int s) { return bars + 64u + 8u * (L::kK + s); };
+    const auto v_full = [&](int s) { return bars + 64u + 8u * (2 * L::kK + s); };
+    const auto v_empty = [&](int s) { return bars + 64u + 8u * (2 * L::kK + L::kV + s); };
+    constexpr uint32_t kSlot = 64 + 16 * (L::kK + L::kV);
+    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + kSlot);
+    int *status = &g_status;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = p.batch * p.q_heads;
+    const int bh = blockIdx.x % heads, h = bh % p.q_heads, b = bh / p.q_heads, kh = h / p.group;
+    const int i0 = (int)((gridDim.x - 1 - blockIdx.x) / heads) * kRows;
+    const int keys = keys_of(p, b);
+    const int kb = first_key(p, i0) / kRows;
+    const int ke = (end_key(p, i0 + kRows < p.q_len ? i0 + kRows : p.q_len, keys) + kRows - 1) / kRows;
+    const int steps = ke > kb ? ke - kb : 0;
+
+    if (threadIdx.x == 0) {
+        acp::mbar_init(q_full, 1); acp::mbar_init(g_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(ds_full, 256); acp::mbar_init(done, 1);
+        acp::mbar_init(fix, 1); acp::mbar_init(s_full(0), 1); acp::mbar_init(s_full(1), 1);
+        for (int s = 0; s < L::kK; ++s) { acp::mbar_init(k_full(s), 1); acp::mbar_init(k_empty(s), 1); }
+        for (int s = 0; s < L::kV; ++s) { acp::mbar_init(v_full(s), 1); acp::mbar_init(v_empty(s), 1); }
+        acp::fence_barrier_init();
+        acp::fence_async_smem();
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = *slot;
+    const uint32_t tD = tmem + 256u, tQ = tmem + 384u;                     // S: columns 0 and 128 in turn
+
+    if (warp == 9) {
+        bool ok = steps > 0;
+        if (ok && lane == 0) {
+            acp::mbar_expect_tx(q_full, L::kTile);
+            load_tile<DP>(base, &mq, q_full, i0, h, b);
+            acp::mbar_expect_tx(g_full, L::kTile);
+            load_tile<DP>(base + L::kTile, &mg, g_full, i0, h, b);
+        }
+        for (int x = 0; x < steps && ok; ++x) {
+            const int row = (kb + x) * kRows, ks = x % L::kK, vs = x % L::kV;
+            const uint32_t kd = base + L::kRingK + ks * L::kTile, vd = base + L::kRingV + vs * L::kTile;
+            ok = wait(k_empty(ks), ((uint32_t)(x / L::kK) & 1u) ^ 1u, 21, status);
+            if (!ok) break;
+            // rows behind the length may hold anything: zeros instead (dS K, and dP where dS is 0)
+            const bool cut = keys < p.k_len && row + kRows > keys;
+            if (!cut) {
+                if (lane == 0) {
+                    acp::mbar_expect_tx(k_full(ks), L::kTile);
+                    load_tile<DP>(kd, &mk, k_full(ks), row, kh, b);
+                }
+                ok = wait(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
+                if (!ok) break;
+                if (lane == 0) {
+                    acp::mbar_expect_tx(v_full(vs), L::kTile);
+                    load_tile<DP>(vd, &mv, v_full(vs), row, kh, b);
+                }
+            } else {                                                      // the last tile of the walk
+                ok = wait(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
+                if (!ok) break;
+                if (lane == 0) {
+                    acp::mbar_expect_tx(fix, 2 * L::kTile);
+                    load_tile<DP>(kd, &mk, fix, row, kh, b);
+                    load_tile<DP>(vd, &mv, fix, row, kh, b);
+                }
+                ok = wait(fix, 0u, 23, status);
+                if (!ok) break;
+                clear_rows<DP>(gen + (kd - base), keys - row);
+                clear_rows<DP>(gen + (vd - base), keys - row);
+                if (lane == 0) { acp::mbar_arrive(k_full(ks)); acp::mbar_arrive(v_full(vs)); }
+            }
+            __syncwarp();
+        }
+    } else if (warp == 8) {
+        if (lane == 0 && steps > 0) {
+            const auto kt = [&](int x) { return base + L::kRingK + (uint32_t)(x % L::kK) * L::kTile; };
+            const auto vt = [&](int x) { return base + L::kRingV + (uint32_t)(x % L::kV) * L::kTile; };
+            const auto scores = [&](int x) {                              // S = Q K^T
+                if (!wait(k_full(x % L::kK), (uint32_t)(x / L::kK) & 1u, 24, status)) return false;
+                fence_after();
+                product_rows<DP>(tmem + 128u * (x & 1), base, kt(x));
+                commit(s_full(x & 1));
+                return true;
+            };
+            const auto grads = [&](int x) {                               // dP = dO V^T
+                if (!wait(v_full(x % L::kV), (uint32_t)(x / L::kV) & 1u, 25, status)) return false;
+                fence_after();
+                product_rows<DP>(tD, base + L::kTile, vt(x));
+                commit(d_full);
+                commit(v_empty(x % L::kV));
+                return true;
+            };
+            bool ok = wait(q_full, 0u, 26, status) && scores(0) && wait(g_full, 0u, 27, status) && grads(0);
+            if (ok && steps > 1) ok = scores(1);
+            for (int x = 0; x < steps && ok; ++x) {
+                ok = wait(ds_full, (uint32_t)x & 1u, 28, status);
+                if (!ok) break;
+                fence_after();
+                product_halves<DP>(tQ, tD, kt(x), x != 0);                // dQ += dS K
+                commit(k_empty(x % L::kK));
+                if (x + 1 < steps) ok = grads(x + 1);
+                if (ok && x + 2 < steps) ok = scores(x + 2);              // its columns were read before dS of this step was written
+            }
+            if (ok) commit(done);
+        }
+    } else if (warp < 8) {
+        const int half = warp >> 2, row = threadIdx.x & 127, i = i0 + row;
+        const uint32_t mine = ((uint32_t)(warp & 3) << 21) + 64u * half;
+        const float c = p.scale * kLog2e;
+        const long long at = ((long long)b * p.q_heads + h) * w.padded + i;        // padded rows exist
+        const float shift = w.shift[at], log_sum = kMask ? w.log_sum[at] : 0.0f, delta = w.delta[at];
+        bool ok = true;
+        for (int x = 0; x < steps; ++x) {
+            ok = wait(s_full(x & 1), (uint32_t)(x / 2) & 1u, 29, status);
+            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            fence_after();
+            uint32_t r[64];
+            ld32(tmem + 128u * (x & 1) + mine, r);
+            ld32(tmem + 128u * (x & 1) + mine + 32u, r + 32);
+            wait_ld();
+            const int j0 = (kb + x) * kRows, first = j0 + 64 * half;
+            if (kMask) {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) {
+                    const float y = sees(p, i, first + e, keys) ? masked_score(p, __uint_as_float(r[e]) * p.scale, b, h, i, first + e) : -CUDART_INF_F;
+                    r[e] = __float_as_uint(y == -CUDART_INF_F ? 0.0f : ex2(fmaf(y - shift, kLog2e, -log_sum)));
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 64; ++e) r[e] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e]), c, -shift)));
+                if (j0 + kRows > keys || (p.causal && j0 + kRows - 1 > i0 + p.offset) || (p.window && j0 <= i0 + kRows - 1 + p.offset - p.window)) {
+                    int lo = 0, hi = keys - first;                                 // visible columns [lo, hi)
+                    if (p.causal && i + p.offset + 1 - first < hi) hi = i + p.offset + 1 - first;
+                    if (p.window) lo = i + p.offset - p.window + 1 - first;
+#pragma unroll
+                    for (int e = 0; e < 64; ++e)
+                        if (e < lo || e >= hi) r[e] = 0u;
+                }
+            }
+            ok = wait(d_full, (uint32_t)x & 1u, 30, status);
+            if (!__all_sync(~0u, ok)) { ok = false; break; }
+            fence_after();
+            uint32_t d[64];
+            ld32(tD + mine, d);
+            ld32(tD + mine + 32u, d + 32);
+            wait_ld();
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t y[8];
+#pragma unroll
+                for (int z = 0; z < 8; ++z) {
+                    const int a = 16 * e + 2 * z;
+                    y[z] = pack2(__uint_as_float(r[a]) * (__uint_as_float(d[a]) - delta), __uint_as_float(r[a + 1]) * (__uint_as_float(d[a + 1]) - delta));
+                }
+                st8(tD + mine + 8u * e, y);
+            }
+            wait_st();
+            fence_before();
+            acp::mbar_arrive(ds_full);
+        }
+        if (ok && steps > 0) {
+            ok = wait(done, 0u, 31, status);
+            ok = __all_sync(~0u, ok);
+            fence_after();
+        }
+        if (ok) {
+            // each half of the warps writes half of the columns
+            __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.dq) + b * p.dq_b + h * p.dq_h + i * p.dq_t;
+#pragma unroll 1
+            for (int x = half * (DP / 64); x < (half + 1) * (DP / 64); ++x) {
+                uint32_t o[32];
+                if (steps > 0) { ld32(tQ + ((uint32_t)(warp & 3) << 21) + 32u * x, o); wait_ld(); }
+                else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) o[e] = 0u;
+                }
+                if (i < p.q_len) store_piece(out, 32 * x, p.head_size, o, p.scale);
+            }
+        }
+    }
+    linger_if_failed(status);
+    fence_before();
+    __syncthreads();
+    if (warp == 8) {
+        fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+    }
+}
+
+}  // namespace tc
+}  // namespace attn
+}  // namespace axs6

@@ -16,6 +16,7 @@ struct View { const void *p; long long b, h, t; };        // (batch, head, token
 struct Params {
     View q, k, v, o, d_o;                   // o: forward's output / backward's input
     void *out, *dq, *dk, *dv;               // written tensors, with the strides below
+    void *o_low;                            // null, or what rounding left of o (bf16), laid out like it
     long long out_b, out_h, out_t, dq_b, dq_h, dq_t, dk_b, dk_h, dk_t, dv_b, dv_h, dv_t;
     float *row_max, *row_sum, *lse;         // (batch, q_heads, q_len)
     float *delta;                           // the same shape, workspace of the backward pass

@@ -247,7 +247,10 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0u;
                 }
-                if (i < p.q_len) store_piece(out, 32 * x, p.head_size, o, inv);
+                if (i < p.q_len) {
+                    store_piece(out, 32 * x, p.head_size, o, inv);
+                    if (p.o_low) store_rest(static_cast<__nv_bfloat16 *>(p.o_low) + (out - static_cast<__nv_bfloat16 *>(p.out)), 32 * x, p.head_size, o, inv);
+                }
             }
             if (i < p.q_len) {
                 const long long at = ((long long)b * p.q_heads + h) * p.q_len + i;

@@ -344,7 +344,6 @@ template <typename T, int DP> static int bwd_t(const Params &p, cudaStream_t st)
 
 int fwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? fwd_t<float, 64>(p, st) : fwd_t<float, 128>(p, st); }
 int bwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? bwd_t<float, 64>(p, st) : bwd_t<float, 128>(p, st); }
-int bwd_bf16_simt(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? bwd_t<__nv_bfloat16, 64>(p, st) : bwd_t<__nv_bfloat16, 128>(p, st); }
 
 }  // namespace attn
 }  // namespace axs6

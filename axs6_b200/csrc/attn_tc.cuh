@@ -80,6 +80,14 @@ template <int DP> __device__ __forceinline__ void product_cols(uint32_t d, uint3
         mma_ts(d, a + 8u * (uint32_t)k, desc(b + (uint32_t)k * 2048u, kBox), instr(DP, 1), acc || k != 0);
 }
 
+// The same with A's columns in two halves, each over the fp32 columns it was made from: tokens 0..63 at column 0, 64..127 at column 64
+template <int DP> __device__ __forceinline__ void product_halves(uint32_t d, uint32_t a, uint32_t b, bool acc)
+{
+#pragma unroll
+    for (int k = 0; k < kRows / 16; ++k)
+        mma_ts(d, a + 64u * (uint32_t)(k / 4) + 8u * (uint32_t)(k % 4), desc(b + (uint32_t)k * 2048u, kBox), instr(DP, 1), acc || k != 0);
+}
+
 #define AXS6_REGS32(r) \
     "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), \
     "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),    \
@@ -151,6 +159,17 @@ __device__ __forceinline__ void store_piece(__nv_bfloat16 *row, int c0, int d, c
                 if (c0 + x < d) row[c0 + x] = __float2bfloat16_rn(__uint_as_float(r[x]) * f);
         }
     }
+}
+
+// What rounding left of the same values, in the same places of another tensor
+__device__ __forceinline__ void store_rest(__nv_bfloat16 *row, int c0, int d, uint32_t *r, float f)
+{
+#pragma unroll
+    for (int e = 0; e < 32; ++e) {
+        const float v = __uint_as_float(r[e]) * f;
+        r[e] = __float_as_uint(v - __bfloat162float(__float2bfloat16_rn(v)));
+    }
+    store_piece(row, c0, d, r, 1.0f);
 }
 
 // On the way out of a kernel in which a wait gave up: loads and products that were issued may still be running; they complete within

@@ -863,7 +863,7 @@ def _attn_strides(t: torch.Tensor):
     return s
 
 
-def _attn_args(tensors: dict, stats, lse, key_lengths, mask, scale: float, causal: bool, window: int) -> "_lib.AttnArgs":
+def _attn_args(tensors: dict, stats, lse, low, key_lengths, mask, scale: float, causal: bool, window: int) -> "_lib.AttnArgs":
     a = _lib.AttnArgs()
     for name, t in tensors.items():
         setattr(a, name, t.data_ptr())
@@ -871,6 +871,7 @@ def _attn_args(tensors: dict, stats, lse, key_lengths, mask, scale: float, causa
     q, k = tensors["q"], tensors["k"]
     a.row_max, a.row_sum = stats[0].data_ptr(), stats[1].data_ptr()
     a.lse = lse.data_ptr() if lse is not None else None
+    a.o_low = low.data_ptr() if low is not None else None
     a.key_lengths = key_lengths.data_ptr() if key_lengths is not None else None
     if mask is not None:
         a.mask = mask.data_ptr()
@@ -927,8 +928,9 @@ def attention_check(q, k, v, key_lengths, mask, scale, causal, window, who: str)
     return mask, scale, 0 if window is None else int(window)
 
 
-def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window: int, want_lse: bool):
-    """-> (o shaped and laid out like q, row statistics (2, batch, heads, queries), lse or None, the operands as read)."""
+def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window: int, want_lse: bool, for_backward: bool = True):
+    """-> (o shaped and laid out like q, row statistics (2, batch, heads, queries), lse or None, the operands as read, what rounding
+    left of o: bf16 with ``for_backward``, else None)."""
     import ctypes
     q, k, v = (_attn_operand(t) for t in (q, k, v))
     dev = q.device
@@ -938,16 +940,17 @@ def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window
     stats = torch.empty((2, *q.shape[:3]), dtype=torch.float32, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
     key_lengths = key_lengths.contiguous() if key_lengths is not None else None
-    a = _attn_args({"q": q, "k": k, "v": v, "o": o}, stats, lse, key_lengths, mask, scale, causal, window)
+    low = torch.empty_strided(o.shape, o.stride(), dtype=o.dtype, device=dev) if for_backward and o.dtype == torch.bfloat16 else None
+    a = _attn_args({"q": q, "k": k, "v": v, "o": o}, stats, lse, low, key_lengths, mask, scale, causal, window)
     with _on(dev):
         ws = _attn_workspace(a, 0, dev)
         st = _lib.load().axs6_attn_fwd(ctypes.byref(a), _stream(dev))
     _lib.check("axs6_attn_fwd", st)
     del ws
-    return o, stats, lse, q, k, v
+    return o, stats, lse, q, k, v, low
 
 
-def attention_bwd(d_o, q, k, v, o, stats, key_lengths, mask, scale: float, causal: bool, window: int):
+def attention_bwd(d_o, q, k, v, o, low, stats, key_lengths, mask, scale: float, causal: bool, window: int):
     """-> (dq, dk, dv), each laid out like the tensor it belongs to."""
     import ctypes
     dev = q.device
@@ -960,7 +963,7 @@ def attention_bwd(d_o, q, k, v, o, stats, key_lengths, mask, scale: float, causa
         grads.append(g)
     key_lengths = key_lengths.contiguous() if key_lengths is not None else None
     a = _attn_args({"q": q, "k": k, "v": v, "o": o, "d_o": d_o, "dq": grads[0], "dk": grads[1], "dv": grads[2]}, stats, None,
-                   key_lengths, mask, scale, causal, window)
+                   low, key_lengths, mask, scale, causal, window)
     with _on(dev):
         ws = _attn_workspace(a, 1, dev)
         st = _lib.load().axs6_attn_bwd(ctypes.byref(a), _stream(dev))

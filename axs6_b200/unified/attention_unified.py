@@ -17,8 +17,8 @@ class _Attention(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, key_lengths, mask, scale, causal, window, want_lse):
-        o, stats, lse, q, k, v = ops.attention_fwd(q, k, v, key_lengths, mask, scale, causal, window, want_lse)
-        ctx.save_for_backward(q, k, v, o, stats, key_lengths, mask)
+        o, stats, lse, q, k, v, low = ops.attention_fwd(q, k, v, key_lengths, mask, scale, causal, window, want_lse, any(ctx.needs_input_grad))
+        ctx.save_for_backward(q, k, v, o, low, stats, key_lengths, mask)
         ctx.call = (scale, causal, window)
         if lse is None:
             return o
@@ -27,8 +27,8 @@ class _Attention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, d_o, *unused):
-        q, k, v, o, stats, key_lengths, mask = ctx.saved_tensors
-        dq, dk, dv = ops.attention_bwd(d_o, q, k, v, o, stats, key_lengths, mask, *ctx.call)
+        q, k, v, o, low, stats, key_lengths, mask = ctx.saved_tensors
+        dq, dk, dv = ops.attention_bwd(d_o, q, k, v, o, low, stats, key_lengths, mask, *ctx.call)
         return dq, dk, dv, None, None, None, None, None, None
 
 

@@ -424,6 +424,9 @@ typedef struct axs6_attn_args {
     int64_t q_strides[3], k_strides[3], v_strides[3], o_strides[3], d_o_strides[3], dq_strides[3], dk_strides[3], dv_strides[3];
     float *row_max, *row_sum;       /* (batch, q_heads, q_len): written by the forward, read by the backward call */
     float *lse;                     /* NULL, or the same shape: log sum exp of a row's scores, -inf where it sees no key */
+    void *o_low;                    /* bf16 tensors: NULL, or like o (its strides): what the rounding of o to bf16 left over, also as bf16.  Written
+                                       by the forward, read by the backward call, whose sums of o * d_o then keep 16 bits: with few visible
+                                       keys their differences from the probabilities' gradients are small */
     const int32_t *key_lengths;     /* NULL, or batch counts on the device: keys from there on are hidden, whatever they hold */
     const void *mask;               /* mask_kind; strides {batch, head, query, key} in elements, 0 where it is shared */
     int64_t mask_strides[4];

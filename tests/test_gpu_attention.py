@@ -193,8 +193,8 @@ def test_what_lies_around_the_outputs_is_left_alone(dtype):
         return buf[:, :, 1:-1, :40]
     torch.empty_like = guarded
     try:
-        o, stats, lse, q, k, v = ops.attention_fwd(q, k, v, None, mask, scale, True, window, True)
-        grads = ops.attention_bwd(g, q, k, v, o, stats, None, mask, scale, True, window)
+        o, stats, lse, q, k, v, low = ops.attention_fwd(q, k, v, None, mask, scale, True, window, True)
+        grads = ops.attention_bwd(g, q, k, v, o, low, stats, None, mask, scale, True, window)
     finally:
         torch.empty_like = real
     assert len(made) == 4
