@@ -6,7 +6,8 @@
 namespace axs6 {
 namespace attn {
 
-int fwd_bf16(const Params &p, cudaStream_t st);
+int fwd_bf16(const Params &p, float *ws, int sms, cudaStream_t st);
+int64_t fwd_bf16_workspace(int64_t batch, int64_t q_heads, int64_t k_heads, int64_t q_len, int64_t k_len, int64_t head_size, int64_t window);
 int bwd_bf16(const Params &p, cudaStream_t st);
 int64_t bwd_bf16_workspace(int64_t heads, int64_t q_len, bool mask);
 
@@ -53,7 +54,9 @@ static int fill(Params &p, const axs6_attn_args &a, bool backward)
 
 static int64_t workspace(const axs6_attn_args &a, bool backward)
 {
-    if (!backward) return 0;
+    const int64_t window = a.window < a.k_len ? a.window : a.k_len;          // as in the call
+    if (!backward)
+        return a.dtype == AXS6_F32 ? 0 : fwd_bf16_workspace(a.batch, a.q_heads, a.k_heads, a.q_len, a.k_len, a.head_size, a.window && !window ? 1 : window);
     return a.dtype == AXS6_F32 ? rows_of(a) * 4 : bwd_bf16_workspace(a.batch * a.q_heads, a.q_len, a.mask_kind != AXS6_MASK_NONE);   // delta, ...
 }
 
@@ -76,8 +79,11 @@ AXS6_API int axs6_attn_fwd(const axs6_attn_args *args, axs6_stream_t stream)
     if (attn::rows_of(*args) == 0) return AXS6_OK;
     const DeviceInfo &d = device_info();
     if (!d.valid || !d.ok) return AXS6_ERR_DEVICE;
+    const int64_t need = attn::workspace(*args, false);
+    if (need && (!args->workspace || args->workspace_bytes < need)) return AXS6_ERR_WORKSPACE;
+    if (!aligned16(args->workspace)) return AXS6_ERR_ALIGN;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    return args->dtype == AXS6_F32 ? attn::fwd_fp32(p, st) : attn::fwd_bf16(p, st);
+    return args->dtype == AXS6_F32 ? attn::fwd_fp32(p, st) : attn::fwd_bf16(p, static_cast<float *>(args->workspace), d.sms, st);
 }
 
 AXS6_API int axs6_attn_bwd(const axs6_attn_args *args, axs6_stream_t stream)

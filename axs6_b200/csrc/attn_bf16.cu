@@ -1,5 +1,6 @@
 // Host side of the tensor-core attention kernels: alignment checks, tensor maps, launches.
 #include "attn_bwd_kernel.cuh"
+#include "attn_few_kernel.cuh"
 #include "attn_fwd_kernel.cuh"
 
 namespace axs6 {
@@ -34,6 +35,50 @@ template <int DP, bool kMask> static int fwd_launch(const Params &p, const CUten
     kernel<<<grid, kFwdThreads, FwdSmem<DP>::kBytes, st>>>(mq, mk, mv, p);
     count_launch();
     return check_launch();
+}
+
+// Whether the few-queries kernel takes a call, and how the keys are cut.  It does when the stacked rows of a key head fit one tile, so that
+// a key tile is read once instead of once a query head, and when the other kernel's CTAs of 256 queries would leave half of the SMs idle.  Chunks:
+// about kFewPerSm CTAs an SM (two are resident; more even out different lengths), whole key tiles each.
+constexpr int kFewPerSm = 4;
+
+struct Plan { bool few; Few f; int64_t rows; };
+
+static Plan plan_of(int64_t batch, int64_t q_heads, int64_t k_heads, int64_t q_len, int64_t k_len, int64_t window, int sms)
+{
+    Plan pl = {};
+    const int64_t group = k_heads ? q_heads / k_heads : 1, rows = q_len * group;
+    const int64_t wide = (q_len + 2 * kRows - 1) / (2 * kRows) * batch * q_heads;
+    pl.few = rows <= kRows || 2 * wide <= sms;
+    pl.rows = batch * k_heads * rows;
+    int64_t span = (k_len + kRows - 1) / kRows;
+    if (window) {                                                  // queries of one tile stand at most this many keys apart
+        const int64_t seen = (window + (kRows + group - 1) / group + kRows - 1) / kRows + 1;
+        if (seen < span) span = seen;
+    }
+    const int64_t tiles = (rows + kRows - 1) / kRows, ctas = tiles * batch * k_heads;
+    int64_t chunks = ctas ? (kFewPerSm * (int64_t)sms + ctas - 1) / ctas : 1;
+    if (chunks > span) chunks = span;
+    if (chunks < 1) chunks = 1;
+    const int64_t chunk = span ? (span + chunks - 1) / chunks : 1;
+    pl.f.row_tiles = (int)tiles; pl.f.chunk = (int)chunk; pl.f.chunks = span ? (int)((span + chunk - 1) / chunk) : 1;
+    return pl;
+}
+
+template <int DP, bool kMask> static int few_launch(const Params &p, Plan &pl, float *ws, const CUtensorMap &mk, const CUtensorMap &mv, cudaStream_t st)
+{
+    const auto kernel = &few_kernel<DP, kMask>;
+    if (!ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), FewSmem<DP>::kBytes)) return AXS6_ERR_LAUNCH;
+    pl.f.out = ws; pl.f.stat = ws + (pl.f.chunks > 1 ? (int64_t)pl.f.chunks * pl.rows * DP : 0);
+    const int64_t grid = (int64_t)p.batch * p.k_heads * pl.f.row_tiles * pl.f.chunks;
+    if (grid > INT32_MAX) return AXS6_ERR_ARG;
+    kernel<<<(unsigned)grid, kFewThreads, FewSmem<DP>::kBytes, st>>>(mk, mv, p, pl.f);
+    count_launch();
+    const int rc = check_launch();
+    if (rc != AXS6_OK || pl.f.chunks == 1) return rc;
+    if (launch_overlapped(true, join_kernel<DP>, (unsigned)((pl.rows + 3) / 4), 128, 0, st, p, pl.f) != cudaSuccess) return AXS6_ERR_LAUNCH;
+    count_launch();
+    return AXS6_OK;
 }
 
 static RowData row_data(const Params &p)
@@ -100,7 +145,15 @@ int bwd_bf16(const Params &p, cudaStream_t st)
     return mask ? bwd_launch<128, true>(p, mq, mk, mv, mg, st) : bwd_launch<128, false>(p, mq, mk, mv, mg, st);
 }
 
-int fwd_bf16(const Params &p, cudaStream_t st)
+int64_t fwd_bf16_workspace(int64_t batch, int64_t q_heads, int64_t k_heads, int64_t q_len, int64_t k_len, int64_t head_size, int64_t window)
+{
+    const DeviceInfo &d = device_info();
+    if (!d.valid || batch * q_heads * q_len == 0) return 0;
+    const tc::Plan pl = tc::plan_of(batch, q_heads, k_heads, q_len, k_len, window, d.sms);
+    return pl.few && pl.f.chunks > 1 ? pl.f.chunks * pl.rows * ((head_size <= 64 ? 64 : 128) + 2) * 4 : 0;
+}
+
+int fwd_bf16(const Params &p, float *ws, int sms, cudaStream_t st)
 {
     using namespace tc;
     if (!aligned_for_tiles(p, false)) return AXS6_ERR_ALIGN;
@@ -112,6 +165,11 @@ int fwd_bf16(const Params &p, cudaStream_t st)
     else if (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b) ||
              !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b)) return AXS6_ERR_DEVICE;
     const bool mask = p.mask_kind != kMaskNone;
+    Plan pl = plan_of(p.batch, p.q_heads, p.k_heads, p.q_len, p.k_len, p.window, sms);
+    if (pl.few) {
+        if (p.head_size <= 64) return mask ? few_launch<64, true>(p, pl, ws, mk, mv, st) : few_launch<64, false>(p, pl, ws, mk, mv, st);
+        return mask ? few_launch<128, true>(p, pl, ws, mk, mv, st) : few_launch<128, false>(p, pl, ws, mk, mv, st);
+    }
     if (p.head_size <= 64) return mask ? fwd_launch<64, true>(p, mq, mk, mv, st) : fwd_launch<64, false>(p, mq, mk, mv, st);
     return mask ? fwd_launch<128, true>(p, mq, mk, mv, st) : fwd_launch<128, false>(p, mq, mk, mv, st);
 }

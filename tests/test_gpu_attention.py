@@ -265,3 +265,24 @@ def test_refusals():
                      (dict(q=torch.randn(1, 1, 4, 129, device="cuda"), k=torch.randn(1, 1, 4, 129, device="cuda"), v=torch.randn(1, 1, 4, 129, device="cuda")), ValueError)]:
         with pytest.raises(err):
             unified.axs_attention_unified(**(dict(q=q, k=k, v=v) | bad))
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Sk,D,window", [(1, 1, 1, 1, 70000, 64, None), (3, 8, 2, 1, 2500, 128, None), (2, 12, 4, 7, 1000, 96, None),
+                                                     (1, 64, 1, 3, 1500, 64, None), (1, 8, 2, 200, 3000, 128, None), (1, 2, 2, 1000, 1000, 64, None),
+                                                     (1, 16, 2, 33, 4000, 64, 500), (1, 4, 1, 400, 300, 72, None), (40, 4, 4, 100, 129, 40, None),
+                                                     (2, 4, 2, 1, 1, 64, None), (5, 130, 1, 1, 900, 64, None)])
+def test_few_queries_stacked_heads_and_cut_keys(causal, B, Hq, Hkv, Sq, Sk, D, window):
+    """One or two tiles of stacked rows, keys in one chunk or many, lengths that leave chunks empty."""
+    if window and not causal:
+        window = None
+    q, k, v, g = tensors(B, Hq, Hkv, Sq, Sk, D, torch.bfloat16, Sq + Sk)
+    compare(q, k, v, g, causal=causal, window=window)
+    lengths = torch.tensor([(Sk * (b + 1) // B if b else 0) for b in range(B)], dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lengths.tolist()):
+        k[b, :, n:] = math.nan
+        v[b, :, n:] = math.nan
+    compare(q, k, v, g, causal=causal, window=window, key_lengths=lengths)
+    mask = torch.rand(1, 1, Sq, Sk, device="cuda") < 0.7
+    k, v = k.nan_to_num(0.0), v.nan_to_num(0.0)
+    compare(q, k, v, g, causal=causal, window=window, mask=mask)
