@@ -51,9 +51,9 @@ static Plan plan_of(int64_t batch, int64_t q_heads, int64_t k_heads, int64_t q_l
     const int64_t wide = (q_len + 2 * kRows - 1) / (2 * kRows) * batch * q_heads;
     pl.few = rows <= kRows || 2 * wide <= sms;
     pl.rows = batch * k_heads * rows;
-    int64_t span = (k_len + kRows - 1) / kRows;
+    int64_t span = (k_len + kKeys - 1) / kKeys;
     if (window) {                                                  // queries of one tile stand at most this many keys apart
-        const int64_t seen = (window + (kRows + group - 1) / group + kRows - 1) / kRows + 1;
+        const int64_t seen = (window + (kRows + group - 1) / group + kKeys - 1) / kKeys + 1;
         if (seen < span) span = seen;
     }
     const int64_t tiles = (rows + kRows - 1) / kRows, ctas = tiles * batch * k_heads;
@@ -161,11 +161,11 @@ int fwd_bf16(const Params &p, float *ws, int sms, cudaStream_t st)
     // without keys nothing is loaded, and the maps of K and V stand in for tensors that need not exist
     const bool none = p.k_len == 0;
     if (!make_map(&mq, p.q.p, p.head_size, p.q_len, p.q_heads, p.batch, p.q.t, p.q.h, p.q.b)) return AXS6_ERR_DEVICE;
-    if (none) { mk = mq; mv = mq; }
-    else if (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b) ||
-             !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b)) return AXS6_ERR_DEVICE;
     const bool mask = p.mask_kind != kMaskNone;
     Plan pl = plan_of(p.batch, p.q_heads, p.k_heads, p.q_len, p.k_len, p.window, sms);
+    if (none) { mk = mq; mv = mq; }
+    else if (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b, kKeys) ||
+             !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b, kKeys)) return AXS6_ERR_DEVICE;
     if (pl.few) {
         if (p.head_size <= 64) return mask ? few_launch<64, true>(p, pl, ws, mk, mv, st) : few_launch<64, false>(p, pl, ws, mk, mv, st);
         return mask ? few_launch<128, true>(p, pl, ws, mk, mv, st) : few_launch<128, false>(p, pl, ws, mk, mv, st);

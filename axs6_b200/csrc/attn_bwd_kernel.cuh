@@ -95,7 +95,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + 48 + 24 * L::kStages);
     int *status = &g_status;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int heads = p.batch * p.k_heads;
     const int bh = blockIdx.x % heads, kh = bh % p.k_heads, b = bh / p.k_heads;
     const int j0 = (int)(blockIdx.x / heads) * kRows;                     // the first keys of a causal call have the longest walk: first
@@ -103,7 +103,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     const int j1 = j0 + kRows < keys ? j0 + kRows : keys;
     const int ib = first_query(p, j0) / kRows;
     const int ie = j0 < keys ? (end_query(p, j1) + kRows - 1) / kRows : 0;
-    const int per_head = ie > ib ? ie - ib : 0, steps = per_head * p.group;
+    const int per_head = uniform(ie > ib ? ie - ib : 0), steps = per_head * p.group;
 
     if (threadIdx.x == 0) {
         acp::mbar_init(kv_full, 1); acp::mbar_init(s_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(p_full, 256); acp::mbar_init(ds_full, 256);
@@ -145,47 +145,64 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
             }
         }
     } else if (warp == 8) {
-        if (lane == 0 && steps > 0) {
+        if (steps > 0) {
+            const bool one = elect();
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kStage; };
             const auto phase = [&](int x) { return (uint32_t)(x / L::kStages) & 1u; };
-            bool ok = wait(kv_full, 0u, 22, status) && wait(q_full(0), 0u, 23, status);
+            bool ok = wait_warp(kv_full, 0u, 22, status) && wait_warp(q_full(0), 0u, 23, status);
             if (ok) {
                 fence_after();
-                product_rows<DP>(tS, base, stage(0));                              // S^T = K Q^T
-                commit(s_full);
-                ok = wait(g_full(0), 0u, 24, status);
-            }
-            if (ok) {
-                fence_after();
-                product_rows<DP>(tD, base + L::kTile, stage(0) + L::kTile);        // dP^T = V dO^T
-                commit(d_full);
-            }
-            for (int x = 0; x < steps && ok; ++x) {
-                ok = wait(p_full, (uint32_t)x & 1u, 25, status);
-                if (!ok) break;
-                fence_after();
-                product_halves<DP>(tV, tS, stage(x) + L::kTile, x != 0);           // dV += P^T dO
-                if (x + 1 < steps) {
-                    ok = wait(q_full((x + 1) % L::kStages), phase(x + 1), 26, status);
-                    if (!ok) break;
-                    fence_after();
-                    product_rows<DP>(tS, base, stage(x + 1));
+                if (one) {
+                    product_rows<DP>(tS, base, stage(0));                              // S^T = K Q^T
                     commit(s_full);
                 }
-                ok = wait(ds_full, (uint32_t)x & 1u, 27, status);
-                if (!ok) break;
+                __syncwarp();
+                ok = wait_warp(g_full(0), 0u, 24, status);
+            }
+            if (ok) {
                 fence_after();
-                product_halves<DP>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
-                commit(empty(x % L::kStages));
-                if (x + 1 < steps) {
-                    ok = wait(g_full((x + 1) % L::kStages), phase(x + 1), 28, status);
-                    if (!ok) break;
-                    fence_after();
-                    product_rows<DP>(tD, base + L::kTile, stage(x + 1) + L::kTile);
+                if (one) {
+                    product_rows<DP>(tD, base + L::kTile, stage(0) + L::kTile);        // dP^T = V dO^T
                     commit(d_full);
                 }
+                __syncwarp();
             }
-            if (ok) commit(done);
+            for (int x = 0; x < steps && ok; ++x) {
+                ok = wait_warp(p_full, (uint32_t)x & 1u, 25, status);
+                if (!ok) break;
+                fence_after();
+                if (one) product_cols<DP, kRows, true>(tV, tS, stage(x) + L::kTile, x != 0);   // dV += P^T dO
+                __syncwarp();
+                if (x + 1 < steps) {
+                    ok = wait_warp(q_full((x + 1) % L::kStages), phase(x + 1), 26, status);
+                    if (!ok) break;
+                    fence_after();
+                    if (one) {
+                        product_rows<DP>(tS, base, stage(x + 1));
+                        commit(s_full);
+                    }
+                    __syncwarp();
+                }
+                ok = wait_warp(ds_full, (uint32_t)x & 1u, 27, status);
+                if (!ok) break;
+                fence_after();
+                if (one) {
+                    product_cols<DP, kRows, true>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
+                    commit(empty(x % L::kStages));
+                }
+                __syncwarp();
+                if (x + 1 < steps) {
+                    ok = wait_warp(g_full((x + 1) % L::kStages), phase(x + 1), 28, status);
+                    if (!ok) break;
+                    fence_after();
+                    if (one) {
+                        product_rows<DP>(tD, base + L::kTile, stage(x + 1) + L::kTile);
+                        commit(d_full);
+                    }
+                    __syncwarp();
+                }
+            }
+            if (ok && one) commit(done);
         }
     } else if (warp < 8) {
         const int half = warp >> 2, row = threadIdx.x & 127, j = j0 + row;
@@ -320,14 +337,14 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + kSlot);
     int *status = &g_status;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int heads = p.batch * p.q_heads;
     const int bh = blockIdx.x % heads, h = bh % p.q_heads, b = bh / p.q_heads, kh = h / p.group;
     const int i0 = (int)((gridDim.x - 1 - blockIdx.x) / heads) * kRows;
     const int keys = keys_of(p, b);
     const int kb = first_key(p, i0) / kRows;
     const int ke = (end_key(p, i0 + kRows < p.q_len ? i0 + kRows : p.q_len, keys) + kRows - 1) / kRows;
-    const int steps = ke > kb ? ke - kb : 0;
+    const int steps = uniform(ke > kb ? ke - kb : 0);
 
     if (threadIdx.x == 0) {
         acp::mbar_init(q_full, 1); acp::mbar_init(g_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(ds_full, 256); acp::mbar_init(done, 1);
@@ -358,7 +375,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
         for (int x = 0; x < steps && ok; ++x) {
             const int row = (kb + x) * kRows, ks = x % L::kK, vs = x % L::kV;
             const uint32_t kd = base + L::kRingK + ks * L::kTile, vd = base + L::kRingV + vs * L::kTile;
-            ok = wait(k_empty(ks), ((uint32_t)(x / L::kK) & 1u) ^ 1u, 21, status);
+            ok = wait_warp(k_empty(ks), ((uint32_t)(x / L::kK) & 1u) ^ 1u, 21, status);
             if (!ok) break;
             // rows behind the length may hold anything: zeros instead (dS K, and dP where dS is 0)
             const bool cut = keys < p.k_len && row + kRows > keys;
@@ -367,21 +384,21 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                     acp::mbar_expect_tx(k_full(ks), L::kTile);
                     load_tile<DP>(kd, &mk, k_full(ks), row, kh, b);
                 }
-                ok = wait(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
+                ok = wait_warp(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
                 if (!ok) break;
                 if (lane == 0) {
                     acp::mbar_expect_tx(v_full(vs), L::kTile);
                     load_tile<DP>(vd, &mv, v_full(vs), row, kh, b);
                 }
             } else {                                                      // the last tile of the walk
-                ok = wait(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
+                ok = wait_warp(v_empty(vs), ((uint32_t)(x / L::kV) & 1u) ^ 1u, 22, status);
                 if (!ok) break;
                 if (lane == 0) {
                     acp::mbar_expect_tx(fix, 2 * L::kTile);
                     load_tile<DP>(kd, &mk, fix, row, kh, b);
                     load_tile<DP>(vd, &mv, fix, row, kh, b);
                 }
-                ok = wait(fix, 0u, 23, status);
+                ok = wait_warp(fix, 0u, 23, status);
                 if (!ok) break;
                 clear_rows<DP>(gen + (kd - base), keys - row);
                 clear_rows<DP>(gen + (vd - base), keys - row);
@@ -390,36 +407,46 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             __syncwarp();
         }
     } else if (warp == 8) {
-        if (lane == 0 && steps > 0) {
+        if (steps > 0) {
+            const bool one = elect();
             const auto kt = [&](int x) { return base + L::kRingK + (uint32_t)(x % L::kK) * L::kTile; };
             const auto vt = [&](int x) { return base + L::kRingV + (uint32_t)(x % L::kV) * L::kTile; };
             const auto scores = [&](int x) {                              // S = Q K^T
-                if (!wait(k_full(x % L::kK), (uint32_t)(x / L::kK) & 1u, 24, status)) return false;
+                if (!wait_warp(k_full(x % L::kK), (uint32_t)(x / L::kK) & 1u, 24, status)) return false;
                 fence_after();
-                product_rows<DP>(tmem + 128u * (x & 1), base, kt(x));
-                commit(s_full(x & 1));
+                if (one) {
+                    product_rows<DP>(tmem + 128u * (x & 1), base, kt(x));
+                    commit(s_full(x & 1));
+                }
+                __syncwarp();
                 return true;
             };
             const auto grads = [&](int x) {                               // dP = dO V^T
-                if (!wait(v_full(x % L::kV), (uint32_t)(x / L::kV) & 1u, 25, status)) return false;
+                if (!wait_warp(v_full(x % L::kV), (uint32_t)(x / L::kV) & 1u, 25, status)) return false;
                 fence_after();
-                product_rows<DP>(tD, base + L::kTile, vt(x));
-                commit(d_full);
-                commit(v_empty(x % L::kV));
+                if (one) {
+                    product_rows<DP>(tD, base + L::kTile, vt(x));
+                    commit(d_full);
+                    commit(v_empty(x % L::kV));
+                }
+                __syncwarp();
                 return true;
             };
-            bool ok = wait(q_full, 0u, 26, status) && scores(0) && wait(g_full, 0u, 27, status) && grads(0);
+            bool ok = wait_warp(q_full, 0u, 26, status) && scores(0) && wait_warp(g_full, 0u, 27, status) && grads(0);
             if (ok && steps > 1) ok = scores(1);
             for (int x = 0; x < steps && ok; ++x) {
-                ok = wait(ds_full, (uint32_t)x & 1u, 28, status);
+                ok = wait_warp(ds_full, (uint32_t)x & 1u, 28, status);
                 if (!ok) break;
                 fence_after();
-                product_halves<DP>(tQ, tD, kt(x), x != 0);                // dQ += dS K
-                commit(k_empty(x % L::kK));
+                if (one) {
+                    product_cols<DP, kRows, true>(tQ, tD, kt(x), x != 0);                // dQ += dS K
+                    commit(k_empty(x % L::kK));
+                }
+                __syncwarp();
                 if (x + 1 < steps) ok = grads(x + 1);
                 if (ok && x + 2 < steps) ok = scores(x + 2);              // its columns were read before dS of this step was written
             }
-            if (ok) commit(done);
+            if (ok && one) commit(done);
         }
     } else if (warp < 8) {
         const int half = warp >> 2, row = threadIdx.x & 127, i = i0 + row;

@@ -7,7 +7,8 @@
 // With a single chunk the result is written at once.
 //
 // Bound: HBM, keys and values once.  Two CTAs live on an SM (half of tensor memory, 97 KB of shared memory each), so that one's products and
-// softmax run under the other's loads, and 128 KB are in flight on an SM.  Warps 0-3: softmax, one thread a row; warps without rows
+// softmax run under the other's loads, and up to 128 KB are in flight on an SM.  Scores are double-buffered in tensor memory: S(j + 1) is
+// issued before P(j) V, so that the softmax of one tile runs under the products of its neighbours.  Warps 0-3: softmax, one thread a row; warps without rows
 // idle (the lanes of P that they would fill hold anything: a row of A reaches only its own row of the product).  Warp 4: products.  Warp 5: loads.
 #pragma once
 #include "attn_tc.cuh"
@@ -19,14 +20,14 @@ namespace tc {
 constexpr int kFewThreads = 192;
 
 struct Few {
-    int row_tiles, chunks, chunk;     // tiles of 128 stacked rows a key head, chunks of the keys, key tiles of a chunk
+    int row_tiles, chunks, chunk;     // tiles of 128 stacked rows a key head, chunks of the keys, key tiles (of 64) of a chunk
     float *out, *stat;                // chunks > 1: (chunk, batch, key head, row, DP) and (chunk, batch, key head, row, 2)
 };
 
 template <int DP> struct FewSmem {
-    static constexpr uint32_t kTile = kBox * (DP / 64);
-    static constexpr int kStages = DP == 64 ? 4 : 2;
-    static constexpr uint32_t kRing = kTile, kBars = kRing + kStages * kTile;
+    static constexpr uint32_t kTile = kKeys * 128 * (DP / 64);
+    static constexpr int kStages = DP == 64 ? 8 : 4;
+    static constexpr uint32_t kRing = kBox * (DP / 64), kBars = kRing + kStages * kTile;
     static constexpr uint32_t kBytes = kBars + 256 + 1024;
 };
 
@@ -39,30 +40,34 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t *gen = raw + (base - smem_u32(raw));
     const uint32_t bars = base + L::kBars;
-    const uint32_t q_full = bars, s_full = bars + 8, p_full = bars + 16, o_full = bars + 24, fix = bars + 32;
-    const auto kv_full = [&](int s) { return bars + 40u + 8u * s; };
-    const auto kv_empty = [&](int s) { return bars + 40u + 8u * (L::kStages + s); };
-    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + 40 + 16 * L::kStages);
+    const uint32_t q_full = bars, fix = bars + 8, o_full = bars + 16;
+    const auto s_full = [&](int x) { return bars + 24u + 8u * x; };
+    const auto p_full = [&](int x) { return bars + 40u + 8u * x; };
+    const auto o_done = [&](int x) { return bars + 56u + 8u * x; };
+    const auto kv_full = [&](int s) { return bars + 72u + 8u * s; };
+    const auto kv_empty = [&](int s) { return bars + 72u + 8u * (L::kStages + s); };
+    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + 72 + 16 * L::kStages);
     int *status = &g_status;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int chunk = blockIdx.x % f.chunks, tile = blockIdx.x / f.chunks % f.row_tiles, bk = blockIdx.x / f.chunks / f.row_tiles;
     const int kh = bk % p.k_heads, b = bk / p.k_heads;
     const int rows = p.q_len * p.group, r0 = tile * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
     const int keys = keys_of(p, b);
-    const int kb = first_key(p, r0 / p.group) / kRows, ke = (end_key(p, (r1 - 1) / p.group + 1, keys) + kRows - 1) / kRows;
+    const int kb = first_key(p, r0 / p.group) / kKeys, ke = (end_key(p, (r1 - 1) / p.group + 1, keys) + kKeys - 1) / kKeys;
     const int from = kb + chunk * f.chunk, to = from + f.chunk < ke ? from + f.chunk : ke;
-    const int steps = to > from ? to - from : 0;
+    const int steps = uniform(to > from ? to - from : 0);
     if (steps == 0 && chunk > 0) return;                                   // the join does not read this chunk
 
     if (threadIdx.x == 0) {
-        acp::mbar_init(q_full, 128); acp::mbar_init(s_full, 1); acp::mbar_init(p_full, (uint32_t)(r1 - r0 + 31) / 32u * 32u); acp::mbar_init(o_full, 1); acp::mbar_init(fix, 1);
+        acp::mbar_init(q_full, 128); acp::mbar_init(o_full, 1); acp::mbar_init(fix, 1);
+        for (int x = 0; x < 2; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(o_done(x), 1); acp::mbar_init(p_full(x), (uint32_t)(r1 - r0 + 31) / 32u * 32u); }
         for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(kv_full(s), 1); acp::mbar_init(kv_empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
     }
     if (warp == 4) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(bars + 40u + 16u * L::kStages) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(bars + 72u + 16u * L::kStages) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
@@ -75,44 +80,55 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
         int s = 0;
         uint32_t ph = 0;
         for (int x = 0; x < 2 * steps && ok; ++x) {
-            const int row = (from + x / 2) * kRows;
-            ok = wait(kv_empty(s), ph ^ 1u, 1, status);
+            const int row = (from + x / 2) * kKeys;
+            ok = wait_warp(kv_empty(s), ph ^ 1u, 1, status);
             if (!ok) break;
             const uint32_t dst = base + L::kRing + s * L::kTile;
-            const bool cut = (x & 1) && keys < p.k_len && row + kRows > keys;
+            const bool cut = (x & 1) && keys < p.k_len && row + kKeys > keys;
             if (lane == 0) {
                 const uint32_t bar = cut ? fix : kv_full(s);
                 acp::mbar_expect_tx(bar, L::kTile);
-                load_tile<DP>(dst, (x & 1) ? &mv : &mk, bar, row, kh, b);
+                load_tile<DP, kKeys>(dst, (x & 1) ? &mv : &mk, bar, row, kh, b);
             }
             if (cut) {
-                ok = wait(fix, 0u, 2, status);
+                ok = wait_warp(fix, 0u, 2, status);
                 if (!ok) break;
-                clear_rows<DP>(gen + (dst - base), keys - row);
+                clear_rows<DP, kKeys>(gen + (dst - base), keys - row);
                 if (lane == 0) acp::mbar_arrive(kv_full(s));
             }
             __syncwarp();
             if (++s == L::kStages) { s = 0; ph ^= 1u; }
         }
     } else if (warp == 4) {
-        if (lane == 0 && steps > 0) {
+        if (steps > 0) {
+            const bool one = elect();
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kTile; };
-            const auto full = [&](int x, int code) { return wait(kv_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, code, status); };
-            bool ok = wait(q_full, 0u, 3, status);
+            const auto full = [&](int x, int code) { return wait_warp(kv_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, code, status); };
+            const auto scores = [&](int j) {
+                if (!full(2 * j, 4)) return false;
+                fence_after();
+                if (one) {
+                    product_rows<DP, kKeys>(tmem + 64u * (j & 1), base, stage(2 * j));
+                    commit(s_full(j & 1));
+                    commit(kv_empty((2 * j) % L::kStages));
+                }
+                __syncwarp();
+                return true;
+            };
+            bool ok = wait_warp(q_full, 0u, 3, status) && scores(0);
             for (int j = 0; j < steps && ok; ++j) {
-                ok = full(2 * j, 4);
+                if (j + 1 < steps) ok = scores(j + 1);                    // over P(j - 1), behind the product that read it
+                ok = ok && full(2 * j + 1, 5) && wait_warp(p_full(j & 1), (uint32_t)(j / 2) & 1u, 6, status);
                 if (!ok) break;
                 fence_after();
-                product_rows<DP>(tmem, base, stage(2 * j));
-                commit(s_full);
-                commit(kv_empty((2 * j) % L::kStages));
-                ok = full(2 * j + 1, 5) && wait(p_full, (uint32_t)j & 1u, 6, status);
-                if (!ok) break;
-                fence_after();
-                product_cols<DP>(tO, tmem, stage(2 * j + 1), j != 0);
-                commit(kv_empty((2 * j + 1) % L::kStages));
+                if (one) {
+                    product_cols<DP, kKeys>(tO, tmem + 64u * (j & 1), stage(2 * j + 1), j != 0);
+                    commit(kv_empty((2 * j + 1) % L::kStages));
+                    commit(o_done(j & 1));
+                }
+                __syncwarp();
             }
-            if (ok) commit(o_full);
+            if (ok && one) commit(o_full);
         }
     } else {
         const int r = r0 + threadIdx.x, i = r / p.group, h = kh * p.group + r % p.group;
@@ -143,36 +159,38 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
         float m = -CUDART_INF_F, l = 0.0f;
         bool ok = true;
         for (int j = 0; j < steps && live; ++j) {
-            ok = wait(s_full, (uint32_t)j & 1u, 7, status);
+            ok = wait(s_full(j & 1), (uint32_t)(j / 2) & 1u, 7, status);
             if (!__all_sync(~0u, ok)) { ok = false; break; }
             fence_after();
-            const int j0 = (from + j) * kRows;
+            const int j0 = (from + j) * kKeys;
+            const uint32_t tS = tmem + lanes + 64u * (j & 1);
             int lo = 0, hi = keys - j0;                                   // visible columns [lo, hi) of this row
             if (p.causal && i + p.offset + 1 - j0 < hi) hi = i + p.offset + 1 - j0;
             if (p.window) lo = i + p.offset - p.window + 1 - j0;
-            uint32_t s[128];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) ld32(tmem + lanes + 32u * x, s + 32 * x);
+            uint32_t s[kKeys];
+            ld32(tS, s);
+            ld32(tS + 32u, s + 32);
             wait_ld();
             if (kMask) {
 #pragma unroll
-                for (int x = 0; x < 128; ++x)
+                for (int x = 0; x < kKeys; ++x)
                     s[x] = __float_as_uint(x >= lo && x < hi && r < r1 ? masked_score(p, __uint_as_float(s[x]) * p.scale, b, h, i, j0 + x) : -CUDART_INF_F);
-            } else if (__any_sync(~0u, lo > 0 || hi < kRows)) {
+            } else if (__any_sync(~0u, lo > 0 || hi < kKeys)) {
 #pragma unroll
-                for (int x = 0; x < 128; ++x)
+                for (int x = 0; x < kKeys; ++x)
                     if (x < lo || x >= hi) s[x] = 0xff800000u;
             }
-            float top = __uint_as_float(s[0]), top1 = __uint_as_float(s[1]);
-#pragma unroll
-            for (int x = 2; x < 128; x += 2) { top = fmaxf(top, __uint_as_float(s[x])); top1 = fmaxf(top1, __uint_as_float(s[x + 1])); }
-            top = fmaxf(top, top1);
+            const float top = row_max<kKeys>(s);
             if (__any_sync(~0u, top > m + slack || (m == -CUDART_INF_F && top > m))) {
                 const float raised = fmaxf(m, top);
                 const float g = m == -CUDART_INF_F ? 0.0f : ex2((m - raised) * c);
                 l *= g;
                 m = raised;
                 if (j > 0) {
+                    // P(j - 1) V is done.  P(j - 3) V on the same barrier was long before: S(j) came behind it, so the parity is unambiguous.
+                    ok = wait(o_done((j - 1) & 1), (uint32_t)((j - 1) / 2) & 1u, 9, status);
+                    if (!__all_sync(~0u, ok)) { ok = false; break; }
+                    fence_after();
 #pragma unroll
                     for (int x = 0; x < DP / 32; ++x) {
                         uint32_t o[32];
@@ -184,22 +202,10 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                     }
                 }
             }
-            const float ref = m == -CUDART_INF_F ? 0.0f : m, shift = -ref * c;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                uint32_t w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const float u = __uint_as_float(s[16 * x + 2 * e]), v = __uint_as_float(s[16 * x + 2 * e + 1]);
-                    const float pu = ex2(kMask ? (u - ref) * c : fmaf(u, c, shift)), pv = ex2(kMask ? (v - ref) * c : fmaf(v, c, shift));
-                    l += pu + pv;
-                    w[e] = pack2(pu, pv);
-                }
-                st8(tmem + lanes + 8u * x, w);
-            }
+            l += exponentials<kKeys, kMask>(s, tS, m == -CUDART_INF_F ? 0.0f : m, c);
             wait_st();
             fence_before();
-            acp::mbar_arrive(p_full);
+            acp::mbar_arrive(p_full(j & 1));
         }
         if (ok && live) {
             if (steps > 0) {
@@ -260,7 +266,7 @@ template <int DP> __global__ void __launch_bounds__(128) join_kernel(const Param
     const int i = r / p.group, h = kh * p.group + r % p.group;
     // chunks that hold keys of this row's tile; the first always wrote
     const int r0 = r / kRows * kRows, r1 = r0 + kRows < rows ? r0 + kRows : rows;
-    const int kb = first_key(p, r0 / p.group) / kRows, ke = (end_key(p, (r1 - 1) / p.group + 1, keys_of(p, b)) + kRows - 1) / kRows;
+    const int kb = first_key(p, r0 / p.group) / kKeys, ke = (end_key(p, (r1 - 1) / p.group + 1, keys_of(p, b)) + kKeys - 1) / kKeys;
     int n = ke > kb ? (ke - kb + f.chunk - 1) / f.chunk : 1;
     if (n > f.chunks) n = f.chunks;
     float m = -CUDART_INF_F;

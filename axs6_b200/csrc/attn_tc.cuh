@@ -17,18 +17,19 @@ namespace tc {
 using acp::smem_u32;
 
 constexpr int kRows = 128;                       // tokens of a tile
+constexpr int kKeys = 64;                        // keys of a tile of the forward kernels
 constexpr uint32_t kBox = 128 * 128;             // bytes of a box
 constexpr uint32_t kWaitPolls = 1u << 20;        // of about a microsecond each, when a poll has to sleep
 
 static __device__ int g_status;                  // 0, or the code of the first wait that gave up (one translation unit includes this)
 
-// false: gave up, or somebody else did
+// false: gave up, or somebody else did.
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code, int *status)
 {
     for (uint32_t i = 0; i < kWaitPolls; ++i) {
         uint32_t ok;
-        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
-                     : "=r"(ok) : "r"(bar), "r"(parity), "r"(1000u) : "memory");
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
         if ((i & 63u) == 63u && *(volatile int *)status != 0) return false;
     }
@@ -36,26 +37,42 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code, in
     return false;
 }
 
+// The same for a loop that a whole warp runs: one answer for all lanes
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, int code, int *status) { return __all_sync(~0u, wait(bar, parity, code, status)); }
+
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void commit(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+// One lane of a warp, the same every time.  The warp that issues the products runs its loop as a whole, so that addresses and descriptors are
+// uniform values, and only the instructions themselves are this lane's (a loop that a single lane runs moved each of the six operand words of
+// a product into a uniform register anew, and that loop, not the tensor cores, set the pace).
+__device__ __forceinline__ bool elect()
 {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}"
-                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+    uint32_t e;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(e));
+    return e != 0;
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc)
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(~0u, v, 0); }
+
+// Descriptors: version 1, 128-byte swizzle, 8-row groups 1024 bytes apart.  The low word holds the address and, for MN-major tiles, the
+// distance of the 64-value boxes; it advances with the contraction.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t addr, uint32_t box) { return ((addr & 0x3FFFFu) >> 4) | ((box >> 4) << 16); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
 {
-    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}"
-                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+    asm volatile("{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh) : "memory");
 }
-// descriptor of a tile: version 1, 128-byte swizzle, 8-row groups 1024 bytes apart; lbo = distance of the 64-value boxes (MN-major only)
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lbo)
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t acc)
 {
-    return (uint64_t)((addr & 0x3FFFFu) >> 4) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(1024u >> 4) << 32) | (1ull << 46) | (2ull << 61);
+    asm volatile("{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+                 " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}"
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(acc), "r"(kDescHigh) : "memory");
 }
 // bf16 operands, fp32 result, M = 128
 __host__ __device__ constexpr uint32_t instr(int n, int b_mn)
@@ -63,29 +80,25 @@ __host__ __device__ constexpr uint32_t instr(int n, int b_mn)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 }
 
-// D (128 x 128) = A B^T over the head's DP values, both tiles K-major
-template <int DP> __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
+// D (128 x kTokens) = A B^T over the head's DP values, tiles at shared addresses `a` (128 rows) and `b` (kTokens rows), both K-major
+template <int DP, int kTokens = kRows> __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
 {
+    const uint32_t al = desc_low(a, 0), bl = desc_low(b, 0);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t off = (uint32_t)(k / 4) * kBox + (uint32_t)(k % 4) * 32u;
-        mma_ss(d, desc(a + off, 0), desc(b + off, 0), instr(128, 0), k != 0);
+        const uint32_t box = (uint32_t)(k / 4), step = (uint32_t)(k % 4) * 2u;
+        mma_ss(d, al + box * (kBox >> 4) + step, bl + box * (kTokens * 128u >> 4) + step, instr(kTokens, 0), k != 0);
     }
 }
-// D (128 x DP) (+)= A B over 128 tokens: A is 128 x 128 bf16 in tensor memory (two values a column), B a tile, MN-major
-template <int DP> __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b, bool acc)
+// D (128 x DP) (+)= A B over kTokens tokens: A is 128 x kTokens bf16 in tensor memory (two values a column), B a tile, MN-major.  kSplit: A's
+// columns in two halves, each over the fp32 columns it was made from: tokens 0..63 at column 0, 64..127 at column 64.
+template <int DP, int kTokens = kRows, bool kSplit = false> __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b, bool acc)
 {
+    const uint32_t bl = desc_low(b, kTokens * 128u);
 #pragma unroll
-    for (int k = 0; k < kRows / 16; ++k)
-        mma_ts(d, a + 8u * (uint32_t)k, desc(b + (uint32_t)k * 2048u, kBox), instr(DP, 1), acc || k != 0);
-}
-
-// The same with A's columns in two halves, each over the fp32 columns it was made from: tokens 0..63 at column 0, 64..127 at column 64
-template <int DP> __device__ __forceinline__ void product_halves(uint32_t d, uint32_t a, uint32_t b, bool acc)
-{
-#pragma unroll
-    for (int k = 0; k < kRows / 16; ++k)
-        mma_ts(d, a + 64u * (uint32_t)(k / 4) + 8u * (uint32_t)(k % 4), desc(b + (uint32_t)k * 2048u, kBox), instr(DP, 1), acc || k != 0);
+    for (int k = 0; k < kTokens / 16; ++k)
+        mma_ts(d, a + (kSplit ? 64u * (uint32_t)(k / 4) + 8u * (uint32_t)(k % 4) : 8u * (uint32_t)k), bl + (uint32_t)k * 128u, instr(DP, 1),
+               k != 0 ? 1u : (uint32_t)acc);
 }
 
 #define AXS6_REGS32(r) \
@@ -121,24 +134,60 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi)
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 
+// Maximum of a row's scores: four chains of three-way maxima
+template <int kN> __device__ __forceinline__ float row_max(const uint32_t *r)
+{
+    float t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = __uint_as_float(r[e]);
+#pragma unroll
+    for (int x = 4; x + 8 <= kN; x += 8)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], fmaxf(__uint_as_float(r[x + e]), __uint_as_float(r[x + 4 + e])));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], __uint_as_float(r[kN - 4 + e]));
+    return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+}
+// exp2(c (s - ref)) of a row's scores, rounded to bf16 pairs into tensor memory from column 0 of `S` on -> their unrounded sum.  Without a mask
+// tensor as one fma a score; with one the difference first, since the scores may be as low as the type goes.
+template <int kN, bool kMask> __device__ __forceinline__ float exponentials(const uint32_t *r, uint32_t S, float ref, float c)
+{
+    const float shift = -ref * c;
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int x = 0; x < kN / 16; ++x) {
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float u = __uint_as_float(r[16 * x + 2 * e]), v = __uint_as_float(r[16 * x + 2 * e + 1]);
+            const float pu = ex2(kMask ? (u - ref) * c : fmaf(u, c, shift)), pv = ex2(kMask ? (v - ref) * c : fmaf(v, c, shift));
+            sum[(2 * e) & 3] += pu;
+            sum[(2 * e + 1) & 3] += pv;
+            w[e] = pack2(pu, pv);
+        }
+        st8(S + 8u * x, w);
+    }
+    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int row, int head, int b)
 {
     asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
                  ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(row), "r"(head), "r"(b) : "memory");
 }
-// 128 tokens of one head; what lies outside the tensor arrives as zeros
-template <int DP> __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int row, int head, int b)
+// The tokens of one head that a box holds (kTokens of them); what lies outside the tensor arrives as zeros
+template <int DP, int kTokens = kRows> __device__ __forceinline__ void load_tile(uint32_t dst, const CUtensorMap *map, uint32_t bar, int row, int head, int b)
 {
 #pragma unroll
-    for (int c = 0; c < DP / 64; ++c) load_box(dst + (uint32_t)c * kBox, map, bar, c * 64, row, head, b);
+    for (int c = 0; c < DP / 64; ++c) load_box(dst + (uint32_t)c * (kTokens * 128u), map, bar, c * 64, row, head, b);
 }
 // A whole warp: zeros into rows [row, 128) of a tile (0 * NaN would reach every row of a product over the tokens), seen by the tensor cores
-template <int DP> __device__ __forceinline__ void clear_rows(uint8_t *tile, int row)
+template <int DP, int kTokens = kRows> __device__ __forceinline__ void clear_rows(uint8_t *tile, int row)
 {
     const int lane = threadIdx.x & 31;
-    for (int i = row * 8 + lane; i < kRows * 8; i += 32)
+    for (int i = row * 8 + lane; i < kTokens * 8; i += 32)
 #pragma unroll
-        for (int c = 0; c < DP / 64; ++c) *reinterpret_cast<uint4 *>(tile + (size_t)c * kBox + (size_t)i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        for (int c = 0; c < DP / 64; ++c) *reinterpret_cast<uint4 *>(tile + (size_t)c * (kTokens * 128) + (size_t)i * 16) = make_uint4(0u, 0u, 0u, 0u);
     acp::fence_async_smem();
     __syncwarp();
 }
@@ -181,15 +230,16 @@ __device__ __forceinline__ void linger_if_failed(int *status)
 }
 
 // ---------------------------------------------------------------------------------------------- host
-// (value, token, head, batch) map of a bf16 tensor, boxes of 64 x 128
-inline bool make_map(CUtensorMap *map, const void *ptr, int d, int64_t tokens, int64_t heads, int64_t batch, int64_t st, int64_t sh, int64_t sb)
+// (value, token, head, batch) map of a bf16 tensor, boxes of 64 values x `rows` tokens
+inline bool make_map(CUtensorMap *map, const void *ptr, int d, int64_t tokens, int64_t heads, int64_t batch, int64_t st, int64_t sh, int64_t sb,
+                     int rows = kRows)
 {
     acp::EncodeTiledFn fn = acp::encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[4] = {(cuuint64_t)d, (cuuint64_t)tokens, (cuuint64_t)heads, (cuuint64_t)batch};
     const cuuint64_t any = (cuuint64_t)((d + 7) / 8 * 16);            // stride of an extent of one: never used, but checked
     const cuuint64_t strides[3] = {tokens > 1 ? (cuuint64_t)st * 2 : any, heads > 1 ? (cuuint64_t)sh * 2 : any, batch > 1 ? (cuuint64_t)sb * 2 : any};
-    const cuuint32_t box[4] = {64, kRows, 1, 1}, es[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, (cuuint32_t)rows, 1, 1}, es[4] = {1, 1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void *>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
