@@ -202,7 +202,10 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
                     }
                 }
             }
-            l += exponentials<kKeys, kMask>(s, tS, m == -CUDART_INF_F ? 0.0f : m, c);
+            Exponentials<kMask> ex(m == -CUDART_INF_F ? 0.0f : m, c);
+#pragma unroll
+            for (int x = 0; x < kKeys / 16; ++x) ex.piece(s + 16 * x, tS + 8u * x);
+            l += ex.sum();
             wait_st();
             fence_before();
             acp::mbar_arrive(p_full(j & 1));

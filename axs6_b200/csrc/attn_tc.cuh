@@ -120,6 +120,18 @@ __device__ __forceinline__ void st32(uint32_t addr, const uint32_t *r)
                  "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]),
                  "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr) : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t *r)
+{
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]) : "r"(addr));
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t *r)
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+                   "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr) : "memory");
+}
 __device__ __forceinline__ void st8(uint32_t addr, const uint32_t *r)
 {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0,%1,%2,%3,%4,%5,%6,%7};"
@@ -148,27 +160,53 @@ template <int kN> __device__ __forceinline__ float row_max(const uint32_t *r)
     for (int e = 0; e < 4; ++e) t[e] = fmaxf(t[e], __uint_as_float(r[kN - 4 + e]));
     return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
-// exp2(c (s - ref)) of a row's scores, rounded to bf16 pairs into tensor memory from column 0 of `S` on -> their unrounded sum.  Without a mask
-// tensor as one fma a score; with one the difference first, since the scores may be as low as the type goes.
-template <int kN, bool kMask> __device__ __forceinline__ float exponentials(const uint32_t *r, uint32_t S, float ref, float c)
-{
-    const float shift = -ref * c;
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int x = 0; x < kN / 16; ++x) {
+// Two fp32 values in one instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void parts(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) { f32x2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c)); return r; }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// exp2(c (s - ref)) of a row's scores, rounded to bf16 pairs into tensor memory, and their unrounded sum.  Without a mask tensor as one fma a
+// score; with one the difference first, since the scores may be as low as the type goes.
+template <bool kMask> struct Exponentials {
+    float ref, c;
+    f32x2 c2, shift2, part[2];
+    __device__ __forceinline__ Exponentials(float ref_, float c_) : ref(ref_), c(c_)
+    {
+        c2 = pair(c, c);
+        shift2 = pair(-ref * c, -ref * c);
+        part[0] = part[1] = pair(0.0f, 0.0f);
+    }
+    // 16 scores into 8 columns
+    __device__ __forceinline__ void piece(const uint32_t *r, uint32_t S)
+    {
         uint32_t w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float u = __uint_as_float(r[16 * x + 2 * e]), v = __uint_as_float(r[16 * x + 2 * e + 1]);
-            const float pu = ex2(kMask ? (u - ref) * c : fmaf(u, c, shift)), pv = ex2(kMask ? (v - ref) * c : fmaf(v, c, shift));
-            sum[(2 * e) & 3] += pu;
-            sum[(2 * e + 1) & 3] += pv;
+            const float u = __uint_as_float(r[2 * e]), v = __uint_as_float(r[2 * e + 1]);
+            float pu, pv;
+            if (kMask) {
+                pu = ex2((u - ref) * c);
+                pv = ex2((v - ref) * c);
+            } else {
+                const f32x2 x = fma2(pair(u, v), c2, shift2);
+                parts(x, pu, pv);
+                pu = ex2(pu);
+                pv = ex2(pv);
+            }
+            part[e & 1] = add2(part[e & 1], pair(pu, pv));
             w[e] = pack2(pu, pv);
         }
-        st8(S + 8u * x, w);
+        st8(S, w);
     }
-    return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-}
+    __device__ __forceinline__ float sum() const
+    {
+        float a, b;
+        parts(add2(part[0], part[1]), a, b);
+        return a + b;
+    }
+};
 
 __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap *map, uint32_t bar, int c0, int row, int head, int b)
 {
