@@ -163,9 +163,10 @@ int fwd_bf16(const Params &p, float *ws, int sms, cudaStream_t st)
     if (!make_map(&mq, p.q.p, p.head_size, p.q_len, p.q_heads, p.batch, p.q.t, p.q.h, p.q.b)) return AXS6_ERR_DEVICE;
     const bool mask = p.mask_kind != kMaskNone;
     Plan pl = plan_of(p.batch, p.q_heads, p.k_heads, p.q_len, p.k_len, p.window, sms);
+    const int box = pl.few ? kKeys : kRows;
     if (none) { mk = mq; mv = mq; }
-    else if (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b, kKeys) ||
-             !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b, kKeys)) return AXS6_ERR_DEVICE;
+    else if (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b, box) ||
+             !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b, box)) return AXS6_ERR_DEVICE;
     if (pl.few) {
         if (p.head_size <= 64) return mask ? few_launch<64, true>(p, pl, ws, mk, mv, st) : few_launch<64, false>(p, pl, ws, mk, mv, st);
         return mask ? few_launch<128, true>(p, pl, ws, mk, mv, st) : few_launch<128, false>(p, pl, ws, mk, mv, st);

@@ -448,7 +448,7 @@ int axs6_attn_fwd(const axs6_attn_args *args, axs6_stream_t stream);
 int axs6_attn_bwd(const axs6_attn_args *args, axs6_stream_t stream);
 
 /* As axs6_gemm_status, for the tensor-core attention kernels: 0 = every wait inside them completed; otherwise the code of a bounded wait
- * that gave up (1..11 forward, 21..39 backward) and the results are invalid.  Synchronises the device and clears the status. */
+ * that gave up (1..10 forward, 21..39 backward) and the results are invalid.  Synchronises the device and clears the status. */
 int axs6_attn_status(void);
 
 /* Bytes of `workspace` for a call with these sizes and type on the current device. */

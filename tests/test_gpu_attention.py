@@ -267,6 +267,29 @@ def test_refusals():
             unified.axs_attention_unified(**(dict(q=q, k=k, v=v) | bad))
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Sk,D,causal,window", [(4, 24, 8, 300, 300, 64, True, None), (2, 40, 40, 257, 1100, 128, False, None),
+                                                            (3, 32, 8, 1100, 1100, 128, True, None), (5, 130, 1, 1, 900, 64, False, None),
+                                                            (2, 48, 16, 700, 700, 80, True, 200), (1, 80, 8, 700, 300, 64, True, None),
+                                                            (2, 64, 64, 513, 1025, 64, False, None)])
+def test_many_heads(B, Hq, Hkv, Sq, Sk, D, causal, window):
+    """Calls that fill the device, one CTA for 256 queries: walks of different and of no length side by side, lengths, masks."""
+    q, k, v, g = tensors(B, Hq, Hkv, Sq, Sk, D, torch.bfloat16, Sq + Sk)
+    compare(q, k, v, g, causal=causal, window=window)
+    compare(q, k, v, g, causal=causal, window=window, mask=torch.rand(B, 1, Sq, Sk, device="cuda") < 0.7)
+    lengths = torch.tensor([(Sk * (b + 1) // B if b else 0) for b in range(B)], dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lengths.tolist()):
+        k[b, :, n:] = math.nan
+        v[b, :, n:] = math.nan
+    compare(q, k, v, g, causal=causal, window=window, key_lengths=lengths)
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    from axs6_b200 import _lib
+    yield
+    assert _lib.load().axs6_attn_status() == 0
+
+
 @pytest.mark.parametrize("causal", [False, True])
 @pytest.mark.parametrize("B,Hq,Hkv,Sq,Sk,D,window", [(1, 1, 1, 1, 70000, 64, None), (3, 8, 2, 1, 2500, 128, None), (2, 12, 4, 7, 1000, 96, None),
                                                      (1, 64, 1, 3, 1500, 64, None), (1, 8, 2, 200, 3000, 128, None), (1, 2, 2, 1000, 1000, 64, None),
