@@ -3,15 +3,17 @@
 //     p_i = softmax(t / T) over the row's used slots        q_j = softmax(z / T) over the whole vocabulary
 //     loss_r = T^2 sum_i p_i (log p_i - log q_(index i))     dz_j = T u_r (q_j - sum_(i: index i = j) p_i)
 // u_r being the upstream gradient of loss_r.  A slot whose index lies outside [0, vocab) or whose teacher logit is -inf is unused;
-// a row without a used slot has loss 0 and gradient 0 and its logits are not read.
+// a row without a used slot has loss 0 and gradient 0, whatever its logits are.
 //
 // Bound: HBM.  Forward reads the logits once (online softmax: every thread keeps a running maximum and the sum relative to it),
 // backward reads them once more and writes the gradient: 3 * rows * vocab * bytes in all.  Nothing of the vocabulary's length is kept
 // between the two, only each row's maximum m and sum s: q = exp((z - m) / T) / s, with the difference taken first so that
-// the exponent carries no rounding of a large log-sum.
+// the exponent carries no rounding of a large log-sum.  Backward takes the rows in the other order, since the last of them are still in L2.
 //
-// One CTA works on one row at a time; 16-byte pieces where the row is aligned, single values up to the first
-// boundary and behind the last.  Sums are fp32 per thread (at most a few hundred terms) and joined in a fixed order.
+// One CTA of 256 threads works on a row, or on a segment of it where rows are few (the segments of a row are a thread-block cluster in the
+// forward kernel, which joins their maxima and sums through distributed shared memory): several CTAs an SM are in different phases,
+// so that the ends of rows hide under the others' loads.  16-byte pieces where the row is aligned, single values up to the first boundary and
+// behind the last.  Sums are fp32 per thread (a few hundred terms) and joined in a fixed order.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
@@ -20,9 +22,10 @@
 namespace axs6 {
 namespace distill {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
-constexpr int kMaxSlots = 1024;
+constexpr int kMaxSlots = 1024, kSlotRounds = kMaxSlots / kThreads;
+constexpr int kMaxSegments = 8;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -32,7 +35,8 @@ struct Params {
     int slots;
     float temperature;
     float *row_loss;        // rows
-    float *stats;           // rows x 2: maximum of z, sum of exp((z - maximum) / T); sum 0 = unused row
+    float4 *stats;          // a row's maximum of z, sum of exp((z - maximum) / T) (0: unused row), the same two of its used teacher logits
+    int segments;           // of a row
     // backward
     void *grad;
     long long ldg;
@@ -57,39 +61,20 @@ template <typename T> __device__ __forceinline__ int head_of(const T *row, long 
     return (long long)h < vocab ? h : (int)vocab;
 }
 
-struct Slots {
-    int index[kMaxSlots];   // -1: unused
-    float p[kMaxSlots];     // teacher logit, then its probability
-};
-
-// Loads a row's slots and turns the teacher's logits into probabilities; sc[0] = sum of exp((t - max) / T) (0: no used slot),
-// sc[1] = max.  Called by the whole CTA; ends with a barrier.
-template <typename Tt>
-__device__ __forceinline__ void load_slots(const Params &p, long long row, Slots &s, float *sc)
+// Pieces [from, to) of a row that segment `seg` has; the values before the first boundary are the first segment's, those behind the last
+// piece the last one's.
+struct Range { int head; long long pieces, from, to; };
+template <typename T> __device__ __forceinline__ Range range_of(const Params &p, const T *row, int seg)
 {
-    const Tt *t = static_cast<const Tt *>(p.t) + row * p.ldt;
-    const long long *ix = p.index + row * p.ldi;
-    for (int i = threadIdx.x; i < p.slots; i += kThreads) {
-        const long long j = ix[i];
-        const float v = to_f(t[i]);
-        const bool used = j >= 0 && j < p.vocab && v != -CUDART_INF_F;
-        s.index[i] = used ? (int)j : -1;
-        s.p[i] = used ? v : -CUDART_INF_F;
-    }
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        const float c = kLog2e / p.temperature;
-        float m = -CUDART_INF_F, sum = 0.0f;
-        for (int i = threadIdx.x; i < p.slots; i += 32) m = fmaxf(m, s.p[i]);
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
-        if (m != -CUDART_INF_F) {
-            for (int i = threadIdx.x; i < p.slots; i += 32) sum += ex2((s.p[i] - m) * c);
-            for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-        }
-        if (threadIdx.x == 0) { sc[0] = sum; sc[1] = m; }
-    }
-    __syncthreads();
+    Range r;
+    r.head = head_of(row, p.vocab);
+    r.pieces = (p.vocab - r.head) / Vec<T>::n;
+    r.from = r.pieces * seg / p.segments;
+    r.to = r.pieces * (seg + 1) / p.segments;
+    return r;
 }
+
+__device__ __forceinline__ int slot_index(const Params &p, long long j, float t) { return j >= 0 && j < p.vocab && t != -CUDART_INF_F ? (int)j : -1; }
 
 // (m, s) of two parts of a row joined: the sum is relative to the maximum.
 __device__ __forceinline__ void join(float &m, float &s, float m2, float s2, float c)
@@ -99,84 +84,148 @@ __device__ __forceinline__ void join(float &m, float &s, float m2, float s2, flo
     m = top;
 }
 
-template <typename T, typename Tt>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const Params p)
+__device__ __forceinline__ uint32_t cluster_address(const void *shared, uint32_t rank)
 {
-    __shared__ Slots slots;
-    __shared__ float sc[2], part[2 * kWarps];
+    uint32_t a;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
+    return a;
+}
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
+}
+
+template <typename T, typename Tt>
+__global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
+{
+    __shared__ int index_s[kMaxSlots];                              // -1: unused
+    __shared__ float teacher_s[kMaxSlots], picked_s[kMaxSlots];
+    __shared__ float part[2 * kWarps];
+    __shared__ float joined[2 * kMaxSegments];                      // in the first CTA of a row: every segment's maximum and sum
+    const long long row = blockIdx.x / p.segments;
+    const int seg = (int)(blockIdx.x % p.segments);
     const float c = kLog2e / p.temperature;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T *z = static_cast<const T *>(p.z) + row * p.ldz;
-        load_slots<Tt>(p, row, slots, sc);
-        if (sc[0] == 0.0f) {                                        // no used slot
-            if (threadIdx.x == 0) { p.row_loss[row] = 0.0f; p.stats[2 * row] = 0.0f; p.stats[2 * row + 1] = 0.0f; }
-            __syncthreads();
-            continue;
-        }
-        float m = -CUDART_INF_F, s = 0.0f;
-        auto one = [&](float v) {
-            if (v > m) { s *= ex2((m - v) * c); m = v; }
-            s += v == -CUDART_INF_F ? 0.0f : ex2((v - m) * c);       // m is finite or +inf here unless v is -inf or NaN
-        };
-        const int head = head_of(z, p.vocab);
-        const long long vecs = (p.vocab - head) / Vec<T>::n;
-        const uint4 *zv = reinterpret_cast<const uint4 *>(z + head);
-        constexpr int kUnroll = 4;
-        long long i = threadIdx.x;
-        auto piece = [&](const Vec<T> &v) {
-            float top = to_f(v.v[0]);
+    const T *z = static_cast<const T *>(p.z) + row * p.ldz;
+    const Tt *tl = static_cast<const Tt *>(p.t) + row * p.ldt;
+    const long long *ix = p.index + row * p.ldi;
+    const Range g = range_of(p, z, seg);
+    const uint4 *zv = reinterpret_cast<const uint4 *>(z + g.head);
+
+    // the first pieces are under way while the slots arrive
+    constexpr int kUnroll = 4;
+    Vec<T> v[kUnroll];
+    long long i = g.from + threadIdx.x;
 #pragma unroll
-            for (int e = 1; e < Vec<T>::n; ++e) top = fmaxf(top, to_f(v.v[e]));
-            if (top > m) { s *= ex2((m - top) * c); m = top; }
-            const float base = m == -CUDART_INF_F ? 0.0f : m;
+    for (int u = 0; u < kUnroll; ++u)
+        if (i + u * kThreads < g.to) v[u].raw = __ldg(zv + i + u * kThreads);
+    bool any = false;
+    int mine[kSlotRounds];
 #pragma unroll
-            for (int e = 0; e < Vec<T>::n; ++e) s += ex2((to_f(v.v[e]) - base) * c);
-        };
-        for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
-            Vec<T> v[kUnroll];
+    for (int x = 0; x < kSlotRounds; ++x) {
+        const int k = threadIdx.x + x * kThreads;
+        mine[x] = -1;
+        if (k >= p.slots) continue;
+        const float t = to_f(tl[k]);
+        mine[x] = slot_index(p, ix[k], t);
+        any |= mine[x] >= 0;
+        if (seg == 0) { index_s[k] = mine[x]; teacher_s[k] = t; }
+    }
+    if (!__syncthreads_or(any)) {                                   // no used slot: the same in all segments of the row
+        if (seg == 0 && threadIdx.x == 0) { p.row_loss[row] = 0.0f; p.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+        return;
+    }
+    float picked[kSlotRounds];
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) v[u].raw = __ldg(zv + i + u * kThreads);
+    for (int x = 0; x < kSlotRounds; ++x) picked[x] = seg == 0 && mine[x] >= 0 ? to_f(z[mine[x]]) : 0.0f;
+
+    float m = -CUDART_INF_F, s = 0.0f;
+    auto one = [&](float w) {
+        if (w > m) { s *= ex2((m - w) * c); m = w; }
+        s += w == -CUDART_INF_F ? 0.0f : ex2((w - m) * c);           // m is finite or +inf here unless w is -inf or NaN
+    };
+    auto piece = [&](const Vec<T> &w) {
+        float top = to_f(w.v[0]);
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) piece(v[u]);
-        }
-        for (; i < vecs; i += kThreads) { Vec<T> v; v.raw = __ldg(zv + i); piece(v); }
-        if ((int)threadIdx.x < head) one(to_f(z[threadIdx.x]));
-        for (long long j = head + vecs * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(to_f(z[j]));
+        for (int e = 1; e < Vec<T>::n; ++e) top = fmaxf(top, to_f(w.v[e]));
+        if (top > m) { s *= ex2((m - top) * c); m = top; }
+        const float base = m == -CUDART_INF_F ? 0.0f : m;
+        float a = 0.0f, b = 0.0f;
+#pragma unroll
+        for (int e = 0; e < Vec<T>::n; e += 2) { a += ex2((to_f(w.v[e]) - base) * c); b += ex2((to_f(w.v[e + 1]) - base) * c); }
+        s += a + b;
+    };
+    for (; i < g.to; i += kUnroll * kThreads) {
+        Vec<T> w[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) w[u] = v[u];
+        const long long next = i + kUnroll * kThreads;
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (next + u * kThreads < g.to) v[u].raw = __ldg(zv + next + u * kThreads);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (i + u * kThreads < g.to) piece(w[u]);
+    }
+    if (seg == 0 && (int)threadIdx.x < g.head) one(to_f(z[threadIdx.x]));
+    if (seg == p.segments - 1)
+        for (long long j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(to_f(z[j]));
+    for (int o = 16; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
+    if ((threadIdx.x & 31) == 0) { part[2 * (threadIdx.x >> 5)] = m; part[2 * (threadIdx.x >> 5) + 1] = s; }
+    if (seg == 0) {
+#pragma unroll
+        for (int x = 0; x < kSlotRounds; ++x)
+            if (threadIdx.x + x * kThreads < p.slots) picked_s[threadIdx.x + x * kThreads] = picked[x];
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        m = -CUDART_INF_F; s = 0.0f;
+        if (threadIdx.x < kWarps) { m = part[2 * threadIdx.x]; s = part[2 * threadIdx.x + 1]; }
         for (int o = 16; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
-        if ((threadIdx.x & 31) == 0) { part[2 * (threadIdx.x >> 5)] = m; part[2 * (threadIdx.x >> 5) + 1] = s; }
-        __syncthreads();
-        if (threadIdx.x < 32) {
-            m = -CUDART_INF_F; s = 0.0f;
-            if (threadIdx.x < kWarps) { m = part[2 * threadIdx.x]; s = part[2 * threadIdx.x + 1]; }
-            for (int o = 16; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
-            // log p_i - log q_i in bits: (t_i - max t) c - log2 sum - (z_i - m) c + log2 s
-            const float lt = log2f(sc[0]), lz = log2f(s), inv = 1.0f / sc[0];
-            float loss = 0.0f;
-            for (int k = threadIdx.x; k < p.slots; k += 32) {
-                if (slots.index[k] < 0) continue;
-                const float a = (slots.p[k] - sc[1]) * c, prob = ex2(a) * inv;
-                if (prob != 0.0f) loss += prob * ((a - lt) - ((to_f(z[slots.index[k]]) - m) * c - lz));
-            }
-            for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(~0u, loss, o);
-            if (threadIdx.x == 0) {
-                p.row_loss[row] = loss * (kLn2 * p.temperature * p.temperature);
-                p.stats[2 * row] = m;
-                p.stats[2 * row + 1] = s;
-            }
+    }
+    if (p.segments > 1) {
+        if (threadIdx.x == 0) {
+            const uint32_t a = cluster_address(joined + 2 * seg, 0);
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(m) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a + 4u), "f"(s) : "memory");
         }
-        __syncthreads();
+        cluster_sync();
+        if (seg == 0 && threadIdx.x < 32) {
+            m = -CUDART_INF_F; s = 0.0f;
+            for (int x = 0; x < p.segments; ++x) join(m, s, joined[2 * x], joined[2 * x + 1], c);
+        }
+    }
+    if (seg == 0 && threadIdx.x < 32) {
+        float tm = -CUDART_INF_F, ts = 0.0f, loss = 0.0f;
+        for (int k = threadIdx.x; k < p.slots; k += 32)
+            if (index_s[k] >= 0) tm = fmaxf(tm, teacher_s[k]);
+        for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, o));
+        for (int k = threadIdx.x; k < p.slots; k += 32)
+            if (index_s[k] >= 0) ts += ex2((teacher_s[k] - tm) * c);
+        for (int o = 16; o; o >>= 1) ts += __shfl_xor_sync(~0u, ts, o);
+        // log p_i - log q_i in bits: (t_i - max t) c - log2 sum t - (z_i - m) c + log2 s
+        const float lt = log2f(ts), lz = log2f(s), inv = 1.0f / ts;
+        for (int k = threadIdx.x; k < p.slots; k += 32) {
+            if (index_s[k] < 0) continue;
+            const float a = (teacher_s[k] - tm) * c, prob = ex2(a) * inv;
+            if (prob != 0.0f) loss += prob * ((a - lt) - ((picked_s[k] - m) * c - lz));
+        }
+        for (int o = 16; o; o >>= 1) loss += __shfl_xor_sync(~0u, loss, o);
+        if (threadIdx.x == 0) {
+            p.row_loss[row] = loss * (kLn2 * p.temperature * p.temperature);
+            p.stats[row] = make_float4(m, s, tm, ts);
+        }
     }
 }
 
 // Sum of the rows' losses, or their mean over the rows with a used slot, in 64 bits and in a fixed order; out[1] = that number of rows.
-__global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, const float *stats, long long rows, int mean, float *out)
+__global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, const float4 *stats, long long rows, int mean, float *out)
 {
     __shared__ double sum_s[32];
     __shared__ long long cnt_s[32];
     pdl_wait();
     double sum = 0.0;
     long long cnt = 0;
-    for (long long i = threadIdx.x; i < rows; i += 1024) { sum += (double)row_loss[i]; cnt += stats[2 * i + 1] != 0.0f; }
+    for (long long i = threadIdx.x; i < rows; i += 1024) { sum += (double)row_loss[i]; cnt += stats[i].y != 0.0f; }
     for (int o = 16; o; o >>= 1) { sum += __shfl_xor_sync(~0u, sum, o); cnt += __shfl_xor_sync(~0u, cnt, o); }
     if ((threadIdx.x & 31) == 0) { sum_s[threadIdx.x >> 5] = sum; cnt_s[threadIdx.x >> 5] = cnt; }
     __syncthreads();
@@ -192,65 +241,73 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, con
 }
 
 template <typename T, typename Tt>
-__global__ void __launch_bounds__(kThreads) backward_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, 5) backward_kernel(const Params p)
 {
-    __shared__ Slots slots;
-    __shared__ float sc[2];
+    __shared__ int index_s[kMaxSlots];
+    __shared__ float prob_s[kMaxSlots];
+    const long long row = p.rows - 1 - blockIdx.x / p.segments;
+    const int seg = (int)(blockIdx.x % p.segments);
     const float c = kLog2e / p.temperature;
-    for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
-        const T *z = static_cast<const T *>(p.z) + row * p.ldz;
-        T *g = static_cast<T *>(p.grad) + row * p.ldg;
-        const float m = p.stats[2 * row], s = p.stats[2 * row + 1];
-        const bool used = s != 0.0f;
-        const float up = p.upstream[row * p.upstream_stride] * p.temperature / (p.count ? *p.count : 1.0f);
-        const float w = used ? up / s : 0.0f;
-        const int head = head_of(g, p.vocab);
-        // 16-byte pieces of both, if the two rows lie alike
-        const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(g)) & 15u) == 0;
-        const long long vecs = alike || !used ? (p.vocab - head) / Vec<T>::n : 0;
-        uint4 *gv = reinterpret_cast<uint4 *>(g + head);
-        auto one = [&](long long j) { from_f(used ? ex2((to_f(z[j]) - m) * c) * w : 0.0f, g[j]); };
-        if (used) {
-            const uint4 *zv = reinterpret_cast<const uint4 *>(z + head);
-            auto piece = [&](const Vec<T> &v, long long at) {
+    const T *z = static_cast<const T *>(p.z) + row * p.ldz;
+    T *grad = static_cast<T *>(p.grad) + row * p.ldg;
+    // segments and boundaries by where the gradient lies; 16-byte pieces of both if the two rows lie alike
+    Range g = range_of(p, grad, seg);
+    const float4 st = p.stats[row];
+    const float m = st.x, s = st.y;
+    const bool used = s != 0.0f, alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) == 0;
+    const float up = p.upstream[row * p.upstream_stride] * p.temperature / (p.count ? *p.count : 1.0f);
+    const float w = used ? up / s : 0.0f;
+    uint4 *gv = reinterpret_cast<uint4 *>(grad + g.head);
+    if (!used) {
+        for (long long i = g.from + threadIdx.x; i < g.to; i += kThreads) __stcs(gv + i, make_uint4(0u, 0u, 0u, 0u));
+    } else if (alike) {
+        const uint4 *zv = reinterpret_cast<const uint4 *>(z + g.head);
+        constexpr int kUnroll = 4;
+        for (long long i = g.from + threadIdx.x; i < g.to; i += kUnroll * kThreads) {
+            Vec<T> v[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u)
+                if (i + u * kThreads < g.to) v[u].raw = __ldg(zv + i + u * kThreads);
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) {
+                if (i + u * kThreads >= g.to) continue;
                 Vec<T> o;
 #pragma unroll
-                for (int e = 0; e < Vec<T>::n; ++e) from_f(ex2((to_f(v.v[e]) - m) * c) * w, o.v[e]);
-                __stcs(gv + at, o.raw);
-            };
-            constexpr int kUnroll = 4;
-            long long i = threadIdx.x;
-            for (; i + (kUnroll - 1) * kThreads < vecs; i += kUnroll * kThreads) {
-                Vec<T> v[kUnroll];
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) v[u].raw = __ldg(zv + i + u * kThreads);
-#pragma unroll
-                for (int u = 0; u < kUnroll; ++u) piece(v[u], i + u * kThreads);
+                for (int e = 0; e < Vec<T>::n; ++e) from_f(ex2((to_f(v[u].v[e]) - m) * c) * w, o.v[e]);
+                __stcs(gv + i + u * kThreads, o.raw);
             }
-            for (; i < vecs; i += kThreads) { Vec<T> v; v.raw = __ldg(zv + i); piece(v, i); }
-        } else {
-            for (long long i = threadIdx.x; i < vecs; i += kThreads) gv[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-        if ((int)threadIdx.x < head) one(threadIdx.x);
-        for (long long j = head + vecs * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(j);
-        if (used) {
-            load_slots<Tt>(p, row, slots, sc);                       // its barriers also order the stores above before those below
-            const float inv = 1.0f / sc[0];
-            // The first slot that names a place writes it, with the probabilities of all the slots that name it in slot order.
-            for (int k = threadIdx.x; k < p.slots; k += kThreads) {
-                const int j = slots.index[k];
-                if (j < 0) continue;
-                float prob = 0.0f;
-                bool first = true;
-                for (int o = 0; o < p.slots; ++o)
-                    if (slots.index[o] == j) {
-                        if (o < k) { first = false; break; }
-                        prob += ex2((slots.p[o] - sc[1]) * c) * inv;
-                    }
-                if (first) from_f((ex2((to_f(z[j]) - m) * c) / s - prob) * up, g[j]);
+    }
+    auto one = [&](long long j) { from_f(used ? ex2((to_f(z[j]) - m) * c) * w : 0.0f, grad[j]); };
+    if (used && !alike)
+        for (long long j = g.head + g.from * Vec<T>::n + threadIdx.x; j < g.head + g.to * Vec<T>::n; j += kThreads) one(j);
+    if (seg == 0 && (int)threadIdx.x < g.head) one(threadIdx.x);
+    if (seg == p.segments - 1)
+        for (long long j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(j);
+    if (!used) return;
+    const Tt *tl = static_cast<const Tt *>(p.t) + row * p.ldt;
+    const long long *ix = p.index + row * p.ldi;
+    const float inv = 1.0f / st.w;
+    for (int k = threadIdx.x; k < p.slots; k += kThreads) {
+        const float t = to_f(tl[k]);
+        const int j = slot_index(p, ix[k], t);
+        index_s[k] = j;
+        prob_s[k] = j >= 0 ? ex2((t - st.z) * c) * inv : 0.0f;
+    }
+    __syncthreads();                                                 // also orders the stores above before those below
+    // The first slot that names a place of this segment writes it, with the probabilities of all the slots that name it in slot order.
+    const long long low = seg == 0 ? 0 : g.head + g.from * Vec<T>::n, high = seg == p.segments - 1 ? p.vocab : g.head + g.to * Vec<T>::n;
+    for (int k = threadIdx.x; k < p.slots; k += kThreads) {
+        const int j = index_s[k];
+        if (j < low || j >= high) continue;                          // -1 among them
+        float prob = 0.0f;
+        bool first = true;
+        for (int o = 0; o < p.slots; ++o)
+            if (index_s[o] == j) {
+                if (o < k) { first = false; break; }
+                prob += prob_s[o];
             }
-            __syncthreads();
-        }
+        if (first) from_f((ex2((to_f(z[j]) - m) * c) / s - prob) * up, grad[j]);
     }
 }
 
@@ -261,12 +318,12 @@ static bool args_ok(const void *z, int dtype, int64_t rows, int64_t vocab, int64
            ldi >= 0 && temperature > 0.0f && temperature <= 3.402823466e38f && (rows == 0 || (z && t && index));
 }
 
-// CTAs: as many as are resident, or one a row.
-static unsigned grid_of(const void *kernel, const DeviceInfo &d, int64_t rows)
+// Segments of a row: doubled while the CTAs would not fill two on every SM and a segment keeps two rounds of a CTA's loads.
+static int segments_of(const DeviceInfo &d, int64_t rows, int64_t vocab, int esize)
 {
-    const int per = cached_occupancy(kernel, kThreads);
-    const int64_t most = (int64_t)d.sms * (per > 0 ? per : 1);
-    return (unsigned)(rows < most ? rows : most);
+    int n = 1;
+    while (n < kMaxSegments && rows * n < 2 * (int64_t)d.sms && vocab * esize / (2 * n) >= 2 * 4 * 16 * kThreads) n *= 2;
+    return n;
 }
 
 }  // namespace distill
@@ -282,18 +339,32 @@ AXS6_API int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64
         reduction > 2 || (rows && (!row_loss || !row_stats)) || (reduction && !reduced))
         return AXS6_ERR_ARG;
     if (slots > kMaxSlots) return AXS6_ERR_UNSUPPORTED;
+    if (!aligned16(row_stats)) return AXS6_ERR_ALIGN;
     const DeviceInfo &d = device_info();
     if (!d.valid || !d.ok) return AXS6_ERR_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     Params p = {};
     p.z = logits; p.t = teacher; p.index = reinterpret_cast<const long long *>(index);
     p.rows = rows; p.vocab = vocab; p.ldz = ld; p.ldt = ld_teacher; p.ldi = ld_index; p.slots = (int)slots; p.temperature = temperature;
-    p.row_loss = row_loss; p.stats = row_stats;
+    p.row_loss = row_loss; p.stats = reinterpret_cast<float4 *>(row_stats);
+    p.segments = segments_of(d, rows, vocab, dtype == AXS6_F32 ? 4 : 2);
+    if (rows * p.segments > INT32_MAX) return AXS6_ERR_ARG;
     if (rows) {
         auto go = [&](auto kernel) {
-            kernel<<<grid_of(reinterpret_cast<const void *>(kernel), d, rows), kThreads, 0, st>>>(p);
+            cudaLaunchConfig_t cfg = {};
+            cfg.gridDim = dim3((unsigned)(rows * p.segments), 1, 1);
+            cfg.blockDim = dim3(kThreads, 1, 1);
+            cfg.stream = st;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim.x = (unsigned)p.segments;
+            attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+            cfg.attrs = attr;
+            cfg.numAttrs = p.segments > 1 ? 1 : 0;
+            const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+            note_cuda_error(e);
             count_launch();
-            return check_launch();
+            return e == cudaSuccess ? AXS6_OK : AXS6_ERR_LAUNCH;
         };
         const int rc = dtype == AXS6_F32
             ? (teacher_dtype == AXS6_F32 ? go(&forward_kernel<float, float>) : go(&forward_kernel<float, __nv_bfloat16>))
@@ -301,7 +372,7 @@ AXS6_API int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64
         if (rc != AXS6_OK) return rc;
     }
     if (reduction) {
-        if (launch_overlapped(true, reduce_kernel, 1, 1024, 0, st, row_loss, row_stats, (long long)rows, reduction == 2, reduced) != cudaSuccess)
+        if (launch_overlapped(true, reduce_kernel, 1, 1024, 0, st, row_loss, p.stats, (long long)rows, reduction == 2, reduced) != cudaSuccess)
             return AXS6_ERR_LAUNCH;
         count_launch();
     }
@@ -319,16 +390,19 @@ AXS6_API int axs6_distill_bwd(const void *logits, int dtype, int64_t rows, int64
         (rows && (!row_stats || !upstream || !grad)))
         return AXS6_ERR_ARG;
     if (slots > kMaxSlots) return AXS6_ERR_UNSUPPORTED;
+    if (!aligned16(row_stats)) return AXS6_ERR_ALIGN;
     if (rows == 0) return AXS6_OK;
     const DeviceInfo &d = device_info();
     if (!d.valid || !d.ok) return AXS6_ERR_DEVICE;
     Params p = {};
     p.z = logits; p.t = teacher; p.index = reinterpret_cast<const long long *>(index);
     p.rows = rows; p.vocab = vocab; p.ldz = ld; p.ldt = ld_teacher; p.ldi = ld_index; p.slots = (int)slots; p.temperature = temperature;
-    p.stats = const_cast<float *>(row_stats); p.grad = grad; p.ldg = ld_grad;
+    p.stats = reinterpret_cast<float4 *>(const_cast<float *>(row_stats)); p.segments = segments_of(d, rows, vocab, dtype == AXS6_F32 ? 4 : 2);
+    if (rows * p.segments > INT32_MAX) return AXS6_ERR_ARG;
+    p.grad = grad; p.ldg = ld_grad;
     p.upstream = upstream; p.upstream_stride = upstream_stride; p.count = count;
     auto go = [&](auto kernel) {
-        kernel<<<grid_of(reinterpret_cast<const void *>(kernel), d, rows), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
+        kernel<<<(unsigned)(rows * p.segments), kThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
         count_launch();
         return check_launch();
     };

@@ -19,7 +19,7 @@ namespace rotary {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 16;         // tokens of a CTA
-constexpr int kTableBytes = 32768;     // cos / sin of its tokens' pairs
+constexpr int kTableBytes = 16384;     // cos / sin of its tokens' pairs
 
 struct Side {                          // q or k: (batch, head, token) strides in elements
     const void *x;
@@ -72,15 +72,23 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void from_f(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
-// kVec: values of a piece.  A unit is kVec pairs (two pieces) of the rotated part or one piece of the rest.
+// kVec: values of a piece.  A unit is two pieces: kVec pairs of the rotated part, or 2 kVec values (at the end kVec) of the rest.
 template <typename T, int kVec>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, 6) rotary_kernel(const Params p)
 {
     typedef typename Piece<kVec * (int)sizeof(T)>::type Raw;
     __shared__ __align__(16) float2 table[kTableBytes / sizeof(float2)];
+    __shared__ long long origin[kMaxTokens][4];                            // of a token in q, q's result, k, k's result
     const long long first = (long long)blockIdx.x * p.tokens_per_cta;
     const int count = (int)(p.total_tokens - first < p.tokens_per_cta ? p.total_tokens - first : p.tokens_per_cta);
 
+    if ((int)threadIdx.x < count) {
+        const long long tok = first + threadIdx.x, b = tok / p.tokens, s = tok - b * p.tokens;
+        origin[threadIdx.x][0] = b * p.side[0].xb + s * p.side[0].xt;
+        origin[threadIdx.x][1] = b * p.side[0].yb + s * p.side[0].yt;
+        origin[threadIdx.x][2] = b * p.side[1].xb + s * p.side[1].xt;
+        origin[threadIdx.x][3] = b * p.side[1].yb + s * p.side[1].yt;
+    }
     for (int i = threadIdx.x; i < count * p.pairs; i += kThreads) {
         const int t = i / p.pairs, pair = i - t * p.pairs;
         const long long tok = first + t, b = tok / p.tokens, s = tok - b * p.tokens;
@@ -90,48 +98,56 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const Params p)
     }
     __syncthreads();
 
-    const int turned = p.pairs / kVec, units = turned + (p.head_size - 2 * p.pairs) / kVec;
-    const int per_token = (p.side[0].heads + p.side[1].heads) * units;
-    for (int i = threadIdx.x; i < count * per_token; i += kThreads) {
-        const int t = i / per_token, r = i - t * per_token;
-        int head = r / units;
-        const int unit = r - head * units;
-        const bool second = head >= p.side[0].heads;
-        const Side &sd = second ? p.side[1] : p.side[0];
-        if (second) head -= p.side[0].heads;
-        const long long tok = first + t, b = tok / p.tokens, s = tok - b * p.tokens;
-        const T *x = static_cast<const T *>(sd.x) + b * sd.xb + head * sd.xh + s * sd.xt;
-        T *y = static_cast<T *>(sd.y) + b * sd.yb + head * sd.yh + s * sd.yt;
+    // (token, head, unit) of this thread's item, advanced by kThreads items at a time in mixed radix
+    const uint32_t heads = (uint32_t)(p.side[0].heads + p.side[1].heads), q_heads = (uint32_t)p.side[0].heads;
+    const uint32_t turned = p.pairs / kVec, rest = (p.head_size - 2 * p.pairs) / kVec, units = turned + (rest + 1) / 2;
+    const uint32_t step_unit = kThreads % units, step_head = kThreads / units % heads, step_token = kThreads / units / heads;
+    uint32_t unit = threadIdx.x % units, head = threadIdx.x / units % heads, t = threadIdx.x / units / heads;
+    const int apart = p.interleaved ? kVec : p.pairs;
+    while (t < (uint32_t)count) {
+        const bool is_k = head >= q_heads;
+        const Side &sd = p.side[is_k];
+        const long long h = is_k ? head - q_heads : head;
+        const T *x = static_cast<const T *>(sd.x) + origin[t][is_k ? 2 : 0] + h * sd.xh;
+        T *y = static_cast<T *>(sd.y) + origin[t][is_k ? 3 : 1] + h * sd.yh;
         if (unit >= turned) {
-            const int at = 2 * p.pairs + (unit - turned) * kVec;
-            *reinterpret_cast<Raw *>(y + at) = *reinterpret_cast<const Raw *>(x + at);
-            continue;
-        }
-        const int at0 = p.interleaved ? unit * 2 * kVec : unit * kVec;
-        const int at1 = p.interleaved ? at0 + kVec : at0 + p.pairs;
-        union Buf { Raw raw[2]; T v[2 * kVec]; } in, out;
-        in.raw[0] = *reinterpret_cast<const Raw *>(x + at0);
-        in.raw[1] = *reinterpret_cast<const Raw *>(x + at1);
-        const float2 *cs = table + t * p.pairs + unit * kVec;
-        if (p.interleaved) {
-#pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                const float a = to_f(in.v[2 * e]), c = to_f(in.v[2 * e + 1]);
-                const float2 w = cs[e];
-                from_f(fmaf(a, w.x, -(c * w.y)), out.v[2 * e]);
-                from_f(fmaf(a, w.y, c * w.x), out.v[2 * e + 1]);
+            const int at = 2 * p.pairs + (int)(unit - turned) * 2 * kVec;
+            const bool two = (unit - turned) * 2 + 1 < rest;
+            const Raw u = *reinterpret_cast<const Raw *>(x + at);
+            if (two) {
+                const Raw w = *reinterpret_cast<const Raw *>(x + at + kVec);
+                *reinterpret_cast<Raw *>(y + at + kVec) = w;
             }
+            *reinterpret_cast<Raw *>(y + at) = u;
         } else {
+            const int at = (int)unit * (p.interleaved ? 2 * kVec : kVec);
+            union Buf { Raw raw[2]; T v[2 * kVec]; } in, out;
+            in.raw[0] = *reinterpret_cast<const Raw *>(x + at);
+            in.raw[1] = *reinterpret_cast<const Raw *>(x + at + apart);
+            const float2 *cs = table + t * p.pairs + unit * kVec;
+            if (p.interleaved) {
 #pragma unroll
-            for (int e = 0; e < kVec; ++e) {
-                const float a = to_f(in.v[e]), c = to_f(in.v[kVec + e]);
-                const float2 w = cs[e];
-                from_f(fmaf(a, w.x, -(c * w.y)), out.v[e]);
-                from_f(fmaf(a, w.y, c * w.x), out.v[kVec + e]);
+                for (int e = 0; e < kVec; ++e) {
+                    const float a = to_f(in.v[2 * e]), c = to_f(in.v[2 * e + 1]);
+                    const float2 w = cs[e];
+                    from_f(fmaf(a, w.x, -(c * w.y)), out.v[2 * e]);
+                    from_f(fmaf(a, w.y, c * w.x), out.v[2 * e + 1]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < kVec; ++e) {
+                    const float a = to_f(in.v[e]), c = to_f(in.v[kVec + e]);
+                    const float2 w = cs[e];
+                    from_f(fmaf(a, w.x, -(c * w.y)), out.v[e]);
+                    from_f(fmaf(a, w.y, c * w.x), out.v[kVec + e]);
+                }
             }
+            *reinterpret_cast<Raw *>(y + at) = out.raw[0];
+            *reinterpret_cast<Raw *>(y + at + apart) = out.raw[1];
         }
-        *reinterpret_cast<Raw *>(y + at0) = out.raw[0];
-        *reinterpret_cast<Raw *>(y + at1) = out.raw[1];
+        unit += step_unit; head += step_head; t += step_token;
+        if (unit >= units) { unit -= units; ++head; }
+        if (head >= heads) { head -= heads; ++t; }
     }
 }
 
@@ -184,7 +200,7 @@ AXS6_API int axs6_rotary(const void *q, void *q_out, int64_t q_heads, const int6
     int vec = 16 / esize;
     while (vec > 1 && !fits(p, vec, esize)) vec >>= 1;
     // Enough tokens for about four units a thread, at most what the table holds, and no fewer CTAs than SMs while tokens last.
-    const int64_t per_token = (q_heads + k_heads) * (p.pairs / vec + (head_size - rotated) / vec);
+    const int64_t per_token = (q_heads + k_heads) * (p.pairs / vec + ((head_size - rotated) / vec + 1) / 2);
     int64_t tpc = (4 * kThreads + per_token - 1) / per_token;
     if (tpc > kMaxTokens) tpc = kMaxTokens;
     if (p.pairs && tpc > kTableBytes / (int64_t)(p.pairs * sizeof(float2))) tpc = kTableBytes / (int64_t)(p.pairs * sizeof(float2));

@@ -784,7 +784,7 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
 # ------------------------------------------------------------------------------------ distillation
 def distill_fwd(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor, temperature: float, reduction: int,
                 who: str = "axs_distillation_unified"):
-    """-> (loss, logits (rows, vocab), teacher (rows, k), index (rows, k), row statistics (rows, 2), count or None): what the
+    """-> (loss, logits (rows, vocab), teacher (rows, k), index (rows, k), row statistics (rows, 4), count or None): what the
     backward call takes.  ``reduction`` 0 none, 1 sum, 2 mean."""
     for t in (logits, teacher, index):
         _check_input(t, who)
@@ -808,7 +808,7 @@ def distill_fwd(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor
         ix = ix.contiguous()
     dev = logits.device
     row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
     reduced = torch.empty(2, dtype=torch.float32, device=dev) if reduction else None
     with _on(dev):
         st = _lib.load().axs6_distill_fwd(z.data_ptr(), _DT[z.dtype], rows, vocab, ldz, t.data_ptr(), _DT[t.dtype], ldt, ix.data_ptr(),

@@ -399,7 +399,8 @@ int axs6_rotary(const void *q, void *q_out, int64_t q_heads, const int64_t *q_st
 /* Distillation from a teacher's top logits.  Row r: p = softmax(teacher / temperature) over the used slots, q = softmax(logits /
  * temperature) over the vocabulary, row_loss = temperature^2 * sum p (log p - log q).  A slot is unused if its index lies outside
  * [0, vocab) or its logit is -inf; a row without a used slot has loss 0 and is not counted.  1 <= slots <= 1024
- * (AXS6_ERR_UNSUPPORTED above).  row_loss: rows floats, row_stats: 2 * rows floats for the backward call.  reduction 0: none,
+ * (AXS6_ERR_UNSUPPORTED above).  row_loss: rows floats, row_stats: 4 * rows floats for the backward call, 16-byte
+ * aligned (AXS6_ERR_ALIGN otherwise).  reduction 0: none,
  * 1: reduced[0] = sum, 2: reduced[0] = mean over the counted rows; reduced[1] = their number, at least 1. */
 int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
                      int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature, int reduction,
