@@ -36,7 +36,7 @@ struct Params {
     float temperature;
     float *row_loss;        // rows
     float4 *stats;          // a row's maximum of z, sum of exp((z - maximum) / T) (0: unused row), the same two of its used teacher logits
-    int segments;           // of a row
+    int segments, shift;    // of a row: a power of two, and its logarithm
     // backward
     void *grad;
     long long ldg;
@@ -51,7 +51,37 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void from_f(float v, float &o) { o = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
-template <typename T> struct Vec { static constexpr int n = 16 / (int)sizeof(T); union { uint4 raw; T v[n]; }; };
+// Two fp32 values in one instruction
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pair(float a, float b) { f32x2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b)); return r; }
+__device__ __forceinline__ void parts(f32x2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) { f32x2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) { f32x2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b)); return r; }
+
+// 16 bytes of a row
+template <typename T> struct Vec {
+    static constexpr int n = 16 / (int)sizeof(T);
+    union { uint4 raw; uint32_t w[4]; T v[n]; };
+    __device__ __forceinline__ f32x2 two(int e) const
+    {
+        if (sizeof(T) == 4) return pair(__uint_as_float(w[(2 * e) & 3]), __uint_as_float(w[(2 * e + 1) & 3]));
+        return pair(__uint_as_float(w[e & 3] << 16), __uint_as_float(w[e & 3] & 0xffff0000u));
+    }
+    __device__ __forceinline__ float top() const
+    {
+        if (sizeof(T) == 4) return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(w);
+        const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    // pair e of values, rounded to the type
+    __device__ __forceinline__ void put(int e, float a, float b)
+    {
+        if (sizeof(T) == 4) { w[(2 * e) & 3] = __float_as_uint(a); w[(2 * e + 1) & 3] = __float_as_uint(b); return; }
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        w[e & 3] = *reinterpret_cast<const uint32_t *>(&h);
+    }
+};
 
 // Values before the first 16-byte boundary of a row (at most vocab).
 template <typename T> __device__ __forceinline__ int head_of(const T *row, long long vocab)
@@ -63,14 +93,14 @@ template <typename T> __device__ __forceinline__ int head_of(const T *row, long 
 
 // Pieces [from, to) of a row that segment `seg` has; the values before the first boundary are the first segment's, those behind the last
 // piece the last one's.
-struct Range { int head; long long pieces, from, to; };
+struct Range { int head, pieces, from, to; };
 template <typename T> __device__ __forceinline__ Range range_of(const Params &p, const T *row, int seg)
 {
     Range r;
     r.head = head_of(row, p.vocab);
-    r.pieces = (p.vocab - r.head) / Vec<T>::n;
-    r.from = r.pieces * seg / p.segments;
-    r.to = r.pieces * (seg + 1) / p.segments;
+    r.pieces = (int)(p.vocab - r.head) / Vec<T>::n;
+    r.from = (r.pieces >> p.shift) * seg;
+    r.to = seg == p.segments - 1 ? r.pieces : r.from + (r.pieces >> p.shift);
     return r;
 }
 
@@ -96,14 +126,14 @@ __device__ __forceinline__ void cluster_sync()
 }
 
 template <typename T, typename Tt>
-__global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, 4) forward_kernel(const Params p)
 {
     __shared__ int index_s[kMaxSlots];                              // -1: unused
     __shared__ float teacher_s[kMaxSlots], picked_s[kMaxSlots];
-    __shared__ float part[2 * kWarps];
+    __shared__ float part[2 * kWarps], teacher_stat[2];
     __shared__ float joined[2 * kMaxSegments];                      // in the first CTA of a row: every segment's maximum and sum
-    const long long row = blockIdx.x / p.segments;
-    const int seg = (int)(blockIdx.x % p.segments);
+    const long long row = blockIdx.x >> p.shift;
+    const int seg = (int)blockIdx.x & (p.segments - 1);
     const float c = kLog2e / p.temperature;
     const T *z = static_cast<const T *>(p.z) + row * p.ldz;
     const Tt *tl = static_cast<const Tt *>(p.t) + row * p.ldt;
@@ -114,7 +144,7 @@ __global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
     // the first pieces are under way while the slots arrive
     constexpr int kUnroll = 4;
     Vec<T> v[kUnroll];
-    long long i = g.from + threadIdx.x;
+    int i = g.from + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u)
         if (i + u * kThreads < g.to) v[u].raw = __ldg(zv + i + u * kThreads);
@@ -138,27 +168,49 @@ __global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
 #pragma unroll
     for (int x = 0; x < kSlotRounds; ++x) picked[x] = seg == 0 && mine[x] >= 0 ? to_f(z[mine[x]]) : 0.0f;
 
-    float m = -CUDART_INF_F, s = 0.0f;
+    // one warp turns the teacher's logits into probabilities while the others begin
+    if (seg == 0 && threadIdx.x >= kThreads - 32) {
+        const int lane = threadIdx.x & 31;
+        float tm = -CUDART_INF_F, ts = 0.0f;
+        for (int k = lane; k < p.slots; k += 32)
+            if (index_s[k] >= 0) tm = fmaxf(tm, teacher_s[k]);
+        for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, o));
+        for (int k = lane; k < p.slots; k += 32)
+            if (index_s[k] >= 0) ts += ex2((teacher_s[k] - tm) * c);
+        for (int o = 16; o; o >>= 1) ts += __shfl_xor_sync(~0u, ts, o);
+        if (lane == 0) { teacher_stat[0] = tm; teacher_stat[1] = ts; }
+    }
+
+    float m = -CUDART_INF_F;
+    f32x2 sum = pair(0.0f, 0.0f);
+    const f32x2 c2 = pair(c, c);
+    auto raise = [&](float top) {
+        if (top > m) {
+            const float f = ex2((m - top) * c);
+            sum = mul2(sum, pair(f, f));
+            m = top;
+        }
+    };
     auto one = [&](float w) {
-        if (w > m) { s *= ex2((m - w) * c); m = w; }
-        s += w == -CUDART_INF_F ? 0.0f : ex2((w - m) * c);           // m is finite or +inf here unless w is -inf or NaN
+        raise(w);
+        sum = add2(sum, pair(w == -CUDART_INF_F ? 0.0f : ex2((w - m) * c), 0.0f));       // m is finite or +inf here unless w is -inf or NaN
     };
     auto piece = [&](const Vec<T> &w) {
-        float top = to_f(w.v[0]);
-#pragma unroll
-        for (int e = 1; e < Vec<T>::n; ++e) top = fmaxf(top, to_f(w.v[e]));
-        if (top > m) { s *= ex2((m - top) * c); m = top; }
+        raise(w.top());
         const float base = m == -CUDART_INF_F ? 0.0f : m;
-        float a = 0.0f, b = 0.0f;
+        const f32x2 back = pair(-base, -base);
 #pragma unroll
-        for (int e = 0; e < Vec<T>::n; e += 2) { a += ex2((to_f(w.v[e]) - base) * c); b += ex2((to_f(w.v[e + 1]) - base) * c); }
-        s += a + b;
+        for (int e = 0; e < Vec<T>::n / 2; ++e) {
+            float a, b;
+            parts(mul2(add2(w.two(e), back), c2), a, b);
+            sum = add2(sum, pair(ex2(a), ex2(b)));
+        }
     };
     for (; i < g.to; i += kUnroll * kThreads) {
         Vec<T> w[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) w[u] = v[u];
-        const long long next = i + kUnroll * kThreads;
+        const int next = i + kUnroll * kThreads;
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u)
             if (next + u * kThreads < g.to) v[u].raw = __ldg(zv + next + u * kThreads);
@@ -168,7 +220,10 @@ __global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
     }
     if (seg == 0 && (int)threadIdx.x < g.head) one(to_f(z[threadIdx.x]));
     if (seg == p.segments - 1)
-        for (long long j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(to_f(z[j]));
+        for (int j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(to_f(z[j]));
+    float s, s_odd;
+    parts(sum, s, s_odd);
+    s += s_odd;
     for (int o = 16; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
     if ((threadIdx.x & 31) == 0) { part[2 * (threadIdx.x >> 5)] = m; part[2 * (threadIdx.x >> 5) + 1] = s; }
     if (seg == 0) {
@@ -178,9 +233,8 @@ __global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
     }
     __syncthreads();
     if (threadIdx.x < 32) {
-        m = -CUDART_INF_F; s = 0.0f;
-        if (threadIdx.x < kWarps) { m = part[2 * threadIdx.x]; s = part[2 * threadIdx.x + 1]; }
-        for (int o = 16; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
+        m = part[2 * (threadIdx.x & (kWarps - 1))]; s = part[2 * (threadIdx.x & (kWarps - 1)) + 1];
+        for (int o = kWarps / 2; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
     }
     if (p.segments > 1) {
         if (threadIdx.x == 0) {
@@ -195,13 +249,8 @@ __global__ void __launch_bounds__(kThreads, 5) forward_kernel(const Params p)
         }
     }
     if (seg == 0 && threadIdx.x < 32) {
-        float tm = -CUDART_INF_F, ts = 0.0f, loss = 0.0f;
-        for (int k = threadIdx.x; k < p.slots; k += 32)
-            if (index_s[k] >= 0) tm = fmaxf(tm, teacher_s[k]);
-        for (int o = 16; o; o >>= 1) tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, o));
-        for (int k = threadIdx.x; k < p.slots; k += 32)
-            if (index_s[k] >= 0) ts += ex2((teacher_s[k] - tm) * c);
-        for (int o = 16; o; o >>= 1) ts += __shfl_xor_sync(~0u, ts, o);
+        const float tm = teacher_stat[0], ts = teacher_stat[1];
+        float loss = 0.0f;
         // log p_i - log q_i in bits: (t_i - max t) c - log2 sum t - (z_i - m) c + log2 s
         const float lt = log2f(ts), lz = log2f(s), inv = 1.0f / ts;
         for (int k = threadIdx.x; k < p.slots; k += 32) {
@@ -225,6 +274,7 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, con
     pdl_wait();
     double sum = 0.0;
     long long cnt = 0;
+#pragma unroll 8
     for (long long i = threadIdx.x; i < rows; i += 1024) { sum += (double)row_loss[i]; cnt += stats[i].y != 0.0f; }
     for (int o = 16; o; o >>= 1) { sum += __shfl_xor_sync(~0u, sum, o); cnt += __shfl_xor_sync(~0u, cnt, o); }
     if ((threadIdx.x & 31) == 0) { sum_s[threadIdx.x >> 5] = sum; cnt_s[threadIdx.x >> 5] = cnt; }
@@ -241,80 +291,109 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, con
 }
 
 template <typename T, typename Tt>
-__global__ void __launch_bounds__(kThreads, 5) backward_kernel(const Params p)
+__global__ void __launch_bounds__(kThreads, 4) backward_kernel(const Params p)
 {
-    __shared__ int index_s[kMaxSlots];
+    __shared__ __align__(16) int index_s[kMaxSlots];
     __shared__ float prob_s[kMaxSlots];
-    const long long row = p.rows - 1 - blockIdx.x / p.segments;
-    const int seg = (int)(blockIdx.x % p.segments);
+    const long long row = p.rows - 1 - (blockIdx.x >> p.shift);
+    const int seg = (int)blockIdx.x & (p.segments - 1);
     const float c = kLog2e / p.temperature;
     const T *z = static_cast<const T *>(p.z) + row * p.ldz;
     T *grad = static_cast<T *>(p.grad) + row * p.ldg;
+    const Tt *tl = static_cast<const Tt *>(p.t) + row * p.ldt;
+    const long long *ix = p.index + row * p.ldi;
     // segments and boundaries by where the gradient lies; 16-byte pieces of both if the two rows lie alike
-    Range g = range_of(p, grad, seg);
+    const Range g = range_of(p, grad, seg);
+    const uint4 *zv = reinterpret_cast<const uint4 *>(z + g.head);
+    const bool alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) == 0;
+    // the first pieces are under way while the statistics and the slots arrive
+    constexpr int kUnroll = 4;
+    Vec<T> v[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u)
+        if (alike && g.from + threadIdx.x + u * kThreads < g.to) v[u].raw = __ldg(zv + g.from + threadIdx.x + u * kThreads);
     const float4 st = p.stats[row];
     const float m = st.x, s = st.y;
-    const bool used = s != 0.0f, alike = ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(grad)) & 15u) == 0;
+    const bool used = s != 0.0f;
     const float up = p.upstream[row * p.upstream_stride] * p.temperature / (p.count ? *p.count : 1.0f);
     const float w = used ? up / s : 0.0f;
+    // the row's slots, and the logits that they name, before the row itself
+    const int low = seg == 0 ? 0 : g.head + g.from * Vec<T>::n, high = seg == p.segments - 1 ? (int)p.vocab : g.head + g.to * Vec<T>::n;
+    int mine[kSlotRounds];
+    float picked[kSlotRounds];
+#pragma unroll
+    for (int x = 0; x < kSlotRounds; ++x) {
+        const int k = threadIdx.x + x * kThreads;
+        mine[x] = -1;
+        picked[x] = 0.0f;
+        if (!used || k >= p.slots) { if (k < (p.slots + 3) / 4 * 4) index_s[k] = -1; continue; }
+        const float t = to_f(tl[k]);
+        const int j = slot_index(p, ix[k], t);
+        index_s[k] = j;
+        prob_s[k] = j >= 0 ? ex2((t - st.z) * c) / st.w : 0.0f;
+        if (j < low || j >= high) continue;                          // -1 among them
+        mine[x] = j;
+        picked[x] = to_f(z[j]);
+    }
     uint4 *gv = reinterpret_cast<uint4 *>(grad + g.head);
     if (!used) {
-        for (long long i = g.from + threadIdx.x; i < g.to; i += kThreads) __stcs(gv + i, make_uint4(0u, 0u, 0u, 0u));
+        for (int i = g.from + threadIdx.x; i < g.to; i += kThreads) __stcs(gv + i, make_uint4(0u, 0u, 0u, 0u));
     } else if (alike) {
-        const uint4 *zv = reinterpret_cast<const uint4 *>(z + g.head);
-        constexpr int kUnroll = 4;
-        for (long long i = g.from + threadIdx.x; i < g.to; i += kUnroll * kThreads) {
-            Vec<T> v[kUnroll];
+        const f32x2 back = pair(-m, -m), c2 = pair(c, c), w2 = pair(w, w);
+        for (int i = g.from + threadIdx.x; i < g.to; i += kUnroll * kThreads) {
+            const int next = i + kUnroll * kThreads;
+            Vec<T> x[kUnroll];
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) x[u] = v[u];
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u)
-                if (i + u * kThreads < g.to) v[u].raw = __ldg(zv + i + u * kThreads);
+                if (next + u * kThreads < g.to) v[u].raw = __ldg(zv + next + u * kThreads);
 #pragma unroll
             for (int u = 0; u < kUnroll; ++u) {
                 if (i + u * kThreads >= g.to) continue;
                 Vec<T> o;
 #pragma unroll
-                for (int e = 0; e < Vec<T>::n; ++e) from_f(ex2((to_f(v[u].v[e]) - m) * c) * w, o.v[e]);
+                for (int e = 0; e < Vec<T>::n / 2; ++e) {
+                    float a, b;
+                    parts(mul2(add2(x[u].two(e), back), c2), a, b);
+                    parts(mul2(pair(ex2(a), ex2(b)), w2), a, b);
+                    o.put(e, a, b);
+                }
                 __stcs(gv + i + u * kThreads, o.raw);
             }
         }
     }
-    auto one = [&](long long j) { from_f(used ? ex2((to_f(z[j]) - m) * c) * w : 0.0f, grad[j]); };
+    auto one = [&](int j) { from_f(used ? ex2((to_f(z[j]) - m) * c) * w : 0.0f, grad[j]); };
     if (used && !alike)
-        for (long long j = g.head + g.from * Vec<T>::n + threadIdx.x; j < g.head + g.to * Vec<T>::n; j += kThreads) one(j);
+        for (int j = g.head + g.from * Vec<T>::n + threadIdx.x; j < g.head + g.to * Vec<T>::n; j += kThreads) one(j);
     if (seg == 0 && (int)threadIdx.x < g.head) one(threadIdx.x);
     if (seg == p.segments - 1)
-        for (long long j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(j);
+        for (int j = g.head + g.pieces * Vec<T>::n + threadIdx.x; j < p.vocab; j += kThreads) one(j);
     if (!used) return;
-    const Tt *tl = static_cast<const Tt *>(p.t) + row * p.ldt;
-    const long long *ix = p.index + row * p.ldi;
-    const float inv = 1.0f / st.w;
-    for (int k = threadIdx.x; k < p.slots; k += kThreads) {
-        const float t = to_f(tl[k]);
-        const int j = slot_index(p, ix[k], t);
-        index_s[k] = j;
-        prob_s[k] = j >= 0 ? ex2((t - st.z) * c) * inv : 0.0f;
-    }
     __syncthreads();                                                 // also orders the stores above before those below
     // The first slot that names a place of this segment writes it, with the probabilities of all the slots that name it in slot order.
-    const long long low = seg == 0 ? 0 : g.head + g.from * Vec<T>::n, high = seg == p.segments - 1 ? p.vocab : g.head + g.to * Vec<T>::n;
-    for (int k = threadIdx.x; k < p.slots; k += kThreads) {
-        const int j = index_s[k];
-        if (j < low || j >= high) continue;                          // -1 among them
+#pragma unroll
+    for (int x = 0; x < kSlotRounds; ++x) {
+        const int j = mine[x], k = threadIdx.x + x * kThreads;
+        if (j < 0) continue;
         float prob = 0.0f;
         bool first = true;
-        for (int o = 0; o < p.slots; ++o)
-            if (index_s[o] == j) {
-                if (o < k) { first = false; break; }
-                prob += prob_s[o];
-            }
-        if (first) from_f((ex2((to_f(z[j]) - m) * c) / s - prob) * up, grad[j]);
+        for (int o = 0; o < p.slots && first; o += 4) {
+            const int4 q = *reinterpret_cast<const int4 *>(index_s + o);
+            if (q.x != j && q.y != j && q.z != j && q.w != j) continue;
+            const int four[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                if (four[y] == j) { prob += prob_s[o + y]; first = first && o + y >= k; }
+        }
+        if (first) from_f((ex2((picked[x] - m) * c) / s - prob) * up, grad[j]);
     }
 }
 
 static bool args_ok(const void *z, int dtype, int64_t rows, int64_t vocab, int64_t ldz, const void *t, int t_dtype, int64_t ldt,
                     const void *index, int64_t ldi, int64_t slots, float temperature)
 {
-    return valid_dtype(dtype) && valid_dtype(t_dtype) && rows >= 0 && vocab >= 1 && vocab < INT32_MAX && slots >= 1 && ldz >= 0 && ldt >= 0 &&
+    return valid_dtype(dtype) && valid_dtype(t_dtype) && rows >= 0 && vocab >= 1 && vocab < INT32_MAX / 2 && slots >= 1 && ldz >= 0 && ldt >= 0 &&
            ldi >= 0 && temperature > 0.0f && temperature <= 3.402823466e38f && (rows == 0 || (z && t && index));
 }
 
@@ -348,6 +427,7 @@ AXS6_API int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64
     p.rows = rows; p.vocab = vocab; p.ldz = ld; p.ldt = ld_teacher; p.ldi = ld_index; p.slots = (int)slots; p.temperature = temperature;
     p.row_loss = row_loss; p.stats = reinterpret_cast<float4 *>(row_stats);
     p.segments = segments_of(d, rows, vocab, dtype == AXS6_F32 ? 4 : 2);
+    while ((1 << p.shift) < p.segments) ++p.shift;
     if (rows * p.segments > INT32_MAX) return AXS6_ERR_ARG;
     if (rows) {
         auto go = [&](auto kernel) {
@@ -398,6 +478,7 @@ AXS6_API int axs6_distill_bwd(const void *logits, int dtype, int64_t rows, int64
     p.z = logits; p.t = teacher; p.index = reinterpret_cast<const long long *>(index);
     p.rows = rows; p.vocab = vocab; p.ldz = ld; p.ldt = ld_teacher; p.ldi = ld_index; p.slots = (int)slots; p.temperature = temperature;
     p.stats = reinterpret_cast<float4 *>(const_cast<float *>(row_stats)); p.segments = segments_of(d, rows, vocab, dtype == AXS6_F32 ? 4 : 2);
+    while ((1 << p.shift) < p.segments) ++p.shift;
     if (rows * p.segments > INT32_MAX) return AXS6_ERR_ARG;
     p.grad = grad; p.ldg = ld_grad;
     p.upstream = upstream; p.upstream_stride = upstream_stride; p.count = count;
