@@ -27,44 +27,52 @@ struct RowData {
     int padded;         // rows of a head
 };
 
-// 16 threads a row, 8 values each
+// 16 threads a row, 8 values each, four rows a thread
 __global__ void __launch_bounds__(256) row_data_kernel(const Params p, const RowData w, int mask)
 {
-    const long long slots = (long long)p.batch * p.q_heads * w.padded;
-    const long long at = (long long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const int part = threadIdx.x & 15;
-    float s = 0.0f;
-    const int i = (int)(at % w.padded), bh = (int)(at / w.padded), h = bh % p.q_heads, b = bh / p.q_heads;
-    const bool real = at < slots && i < p.q_len;
-    if (real) {
-        const __nv_bfloat16 *o = static_cast<const __nv_bfloat16 *>(p.o.p) + b * p.o.b + h * p.o.h + i * p.o.t;
-        const __nv_bfloat16 *g = static_cast<const __nv_bfloat16 *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h + i * p.d_o.t;
-        const __nv_bfloat16 *low = p.o_low ? static_cast<const __nv_bfloat16 *>(p.o_low) + (o - static_cast<const __nv_bfloat16 *>(p.o.p)) : nullptr;
-        const int c = part * 8;
-        if (c + 8 <= p.head_size) {
-            const uint4 x = *reinterpret_cast<const uint4 *>(o + c), y = *reinterpret_cast<const uint4 *>(g + c);
-            const uint4 t = low ? *reinterpret_cast<const uint4 *>(low + c) : make_uint4(0u, 0u, 0u, 0u);
-            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w}, ts[4] = {t.x, t.y, t.z, t.w};
+    const uint32_t tiles = (uint32_t)w.padded / 64u;                       // a CTA has 64 rows of one head
+    const uint32_t bh = blockIdx.x / tiles, h = bh % (uint32_t)p.q_heads, b = bh / (uint32_t)p.q_heads;
+    const int first = (int)(blockIdx.x - bh * tiles) * 64 + (int)(threadIdx.x >> 4), part = threadIdx.x & 15, c = part * 8;
+    const __nv_bfloat16 *o = static_cast<const __nv_bfloat16 *>(p.o.p) + b * p.o.b + h * p.o.h;
+    const __nv_bfloat16 *g = static_cast<const __nv_bfloat16 *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
+    const __nv_bfloat16 *low = p.o_low ? static_cast<const __nv_bfloat16 *>(p.o_low) + (o - static_cast<const __nv_bfloat16 *>(p.o.p)) : nullptr;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    const bool whole = c + 8 <= p.head_size;
+    uint4 x[4], y[4], t[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s = fmaf(__uint_as_float(xs[e] << 16) + __uint_as_float(ts[e] << 16), __uint_as_float(ys[e] << 16), s);
-                s = fmaf(__uint_as_float(xs[e] & 0xffff0000u) + __uint_as_float(ts[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), s);
-            }
-        } else {
-            for (int e = c; e < p.head_size; ++e) s = fmaf(__bfloat162float(o[e]) + (low ? __bfloat162float(low[e]) : 0.0f), __bfloat162float(g[e]), s);
-        }
+    for (int n = 0; n < 4; ++n) {
+        const int i = first + 16 * n;
+        const bool here = whole && i < p.q_len;
+        x[n] = here ? *reinterpret_cast<const uint4 *>(o + i * p.o.t + c) : none;
+        y[n] = here ? *reinterpret_cast<const uint4 *>(g + i * p.d_o.t + c) : none;
+        t[n] = here && low ? *reinterpret_cast<const uint4 *>(low + i * p.o.t + c) : none;
     }
-    for (int x = 8; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
-    if (part == 0 && at < slots) {
-        float shift = mask ? 0.0f : CUDART_INF_F, log_sum = CUDART_INF_F;
-        if (real) {
-            const long long src = (long long)bh * p.q_len + i;
-            const float m = p.row_max[src], l = p.row_sum[src];
-            if (l != 0.0f) { log_sum = log2f(l); shift = mask ? m : fmaf(m, kLog2e, log_sum); }
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int i = first + 16 * n;
+        const uint32_t xs[4] = {x[n].x, x[n].y, x[n].z, x[n].w}, ys[4] = {y[n].x, y[n].y, y[n].z, y[n].w}, ts[4] = {t[n].x, t[n].y, t[n].z, t[n].w};
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            s = fmaf(__uint_as_float(xs[e] << 16) + __uint_as_float(ts[e] << 16), __uint_as_float(ys[e] << 16), s);
+            s = fmaf(__uint_as_float(xs[e] & 0xffff0000u) + __uint_as_float(ts[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), s);
         }
-        w.shift[at] = shift;
-        if (mask) w.log_sum[at] = log_sum;
-        w.delta[at] = s;
+        if (!whole && i < p.q_len)
+            for (int e = c; e < p.head_size; ++e)
+                s = fmaf(__bfloat162float(o[i * p.o.t + e]) + (low ? __bfloat162float(low[i * p.o.t + e]) : 0.0f), __bfloat162float(g[i * p.d_o.t + e]), s);
+        for (int z = 8; z; z >>= 1) s += __shfl_xor_sync(~0u, s, z);
+        if (part == 0) {
+            float shift = mask ? 0.0f : CUDART_INF_F, log_sum = CUDART_INF_F;
+            if (i < p.q_len) {
+                const long long src = (long long)bh * p.q_len + i;
+                const float m = p.row_max[src], l = p.row_sum[src];
+                if (l != 0.0f) { log_sum = log2f(l); shift = mask ? m : fmaf(m, kLog2e, log_sum); }
+            }
+            const long long at = (long long)bh * w.padded + i;
+            w.shift[at] = shift;
+            if (mask) w.log_sum[at] = log_sum;
+            w.delta[at] = s;
+        }
     }
 }
 
@@ -171,7 +179,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 ok = wait_warp(p_full, (uint32_t)x & 1u, 25, status);
                 if (!ok) break;
                 fence_after();
-                if (one) product_cols<DP, kRows, true>(tV, tS, stage(x) + L::kTile, x != 0);   // dV += P^T dO
+                if (one) product_cols<DP, kRows, 64>(tV, tS, stage(x) + L::kTile, x != 0);   // dV += P^T dO
                 __syncwarp();
                 if (x + 1 < steps) {
                     ok = wait_warp(q_full((x + 1) % L::kStages), phase(x + 1), 26, status);
@@ -187,7 +195,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 if (!ok) break;
                 fence_after();
                 if (one) {
-                    product_cols<DP, kRows, true>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
+                    product_cols<DP, kRows, 64>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
                     commit(empty(x % L::kStages));
                 }
                 __syncwarp();
@@ -439,7 +447,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                 if (!ok) break;
                 fence_after();
                 if (one) {
-                    product_cols<DP, kRows, true>(tQ, tD, kt(x), x != 0);                // dQ += dS K
+                    product_cols<DP, kRows, 64>(tQ, tD, kt(x), x != 0);                // dQ += dS K
                     commit(k_empty(x % L::kK));
                 }
                 __syncwarp();

@@ -158,7 +158,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 if (!ok) break;
                 fence_after();
                 if (one) {
-                    product_cols<DP, kRows, true>(tO(t), tS(u % kBufs), stage(2 * j + 1), j != 0);
+                    product_cols<DP, kRows, 64>(tO(t), tS(u % kBufs), stage(2 * j + 1), j != 0);
                     commit(j + 1 == (t ? n1 : n0) ? o_full(t) : o_done(t, j));
                     if (last_of_step(u)) commit(kv_empty((2 * j + 1) % L::kStages));
                 }

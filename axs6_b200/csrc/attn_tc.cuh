@@ -90,14 +90,14 @@ template <int DP, int kTokens = kRows> __device__ __forceinline__ void product_r
         mma_ss(d, al + box * (kBox >> 4) + step, bl + box * (kTokens * 128u >> 4) + step, instr(kTokens, 0), k != 0);
     }
 }
-// D (128 x DP) (+)= A B over kTokens tokens: A is 128 x kTokens bf16 in tensor memory (two values a column), B a tile, MN-major.  kSplit: A's
-// columns in two halves, each over the fp32 columns it was made from: tokens 0..63 at column 0, 64..127 at column 64.
-template <int DP, int kTokens = kRows, bool kSplit = false> __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b, bool acc)
+// D (128 x DP) (+)= A B over kTokens tokens: A is 128 x kTokens bf16 in tensor memory (two values a column), B a tile, MN-major.  kGroup: A's
+// columns in groups of so many tokens, each over the fp32 columns it was made from: token g * kGroup at column g * kGroup.
+template <int DP, int kTokens = kRows, int kGroup = kTokens> __device__ __forceinline__ void product_cols(uint32_t d, uint32_t a, uint32_t b, bool acc)
 {
     const uint32_t bl = desc_low(b, kTokens * 128u);
 #pragma unroll
     for (int k = 0; k < kTokens / 16; ++k)
-        mma_ts(d, a + (kSplit ? 64u * (uint32_t)(k / 4) + 8u * (uint32_t)(k % 4) : 8u * (uint32_t)k), bl + (uint32_t)k * 128u, instr(DP, 1),
+        mma_ts(d, a + (uint32_t)(k * 16 / kGroup * kGroup) + 8u * (uint32_t)(k % (kGroup / 16)), bl + (uint32_t)k * 128u, instr(DP, 1),
                k != 0 ? 1u : (uint32_t)acc);
 }
 
