@@ -138,8 +138,8 @@ int bwd_bf16(const Params &p, cudaStream_t st)
                   !make_map(&mg, p.d_o.p, p.head_size, p.q_len, p.q_heads, p.batch, p.d_o.t, p.d_o.h, p.d_o.b))) return AXS6_ERR_DEVICE;
     if (!no_k && (!make_map(&mk, p.k.p, p.head_size, p.k_len, p.k_heads, p.batch, p.k.t, p.k.h, p.k.b) ||
                   !make_map(&mv, p.v.p, p.head_size, p.k_len, p.k_heads, p.batch, p.v.t, p.v.h, p.v.b))) return AXS6_ERR_DEVICE;
-    if (no_q) { mq = mk; mg = mk; }
-    if (no_k) { mk = mq; mv = mq; }
+    if (no_q) mq = mg = mk;
+    if (no_k) mk = mv = mq;
     const bool mask = p.mask_kind != kMaskNone;
     if (p.head_size <= 64) return mask ? bwd_launch<64, true>(p, mq, mk, mv, mg, st) : bwd_launch<64, false>(p, mq, mk, mv, mg, st);
     return mask ? bwd_launch<128, true>(p, mq, mk, mv, mg, st) : bwd_launch<128, false>(p, mq, mk, mv, mg, st);

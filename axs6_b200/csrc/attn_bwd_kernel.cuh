@@ -4,11 +4,16 @@
 // queries (dQ).  That is 7 products a tile pair instead of the 5 that one kernel would need, and in return every output has one writer:
 // no fp32 copy of dQ in memory, no atomics, the same bits every time.  P and dS are rounded to bf16 as operands; everything else is fp32.
 //
-// Both kernels: warps 0-7 do the elementwise part (row = lane of tensor memory, warps 0-3 columns 0..63, warps 4-7 columns 64..127, 64 values
-// a thread), warp 8 issues the products, warp 9 loads.  P and dS go back to tensor memory over the columns they came from and are the
-// A operands of the next products, so shared memory holds nothing but loaded tiles.
+// Both kernels: warps 0-15 do the elementwise part (row = lane of tensor memory), warp 16 issues the products, warp 17 loads.  P and dS go back
+// to tensor memory over fp32 columns that have been read and are the A operands of the next products, so shared memory holds nothing but
+// loaded tiles.  Within a step the probabilities need S, dS needs dP and the next products need both: a chain during which either the
+// exponential unit or the tensor cores idle.  Where tensor memory has room for a second S, the warps are two sets of eight that take the even
+// and the odd steps: dQ (S, S, dP, dQ), and dK, dV at D = 64 (S, S, dP, dK, dV; P and dS share the columns of S, so that dP is free as
+// soon as it is read).  dK, dV at D = 128 has one set of sixteen (S, dP, dK, dV; P over S, dS over dP).  Every barrier that a set waits on
+// is its own: with one for both, a parity wait could not tell a step from the one before the other set's.
 //
-// Bound: tensor cores, 4 (dK, dV) and 3 (dQ) products of 512 clocks a 128 x 128 tile at D = 128; exp2 takes 1024 clocks a tile in each.
+// Bound: tensor cores.  An M = 128, K = 16 product takes 64 clocks for any N up to 128: per 128 x 128 tile dK and dV 2048 clocks at D = 128 and
+// 1536 at D = 64, dQ 1536 and 1024; exp2 takes 1024 in each.  (Two sets at D = 128 with S and dP for 64 queries at a time: 3072, and slower.)
 #pragma once
 #include "attn_tc.cuh"
 
@@ -16,7 +21,9 @@ namespace axs6 {
 namespace attn {
 namespace tc {
 
-constexpr int kBwdThreads = 384;
+constexpr int kBwdThreads = 640;
+// Registers: launched with 96 a thread, 5 x 96 = 480; 112 for the four warpgroups that hold up to 64 probabilities a thread, 32 for the last
+constexpr int kBwdRegsMore = 112, kBwdRegsLess = 32;
 
 // Per row: what the probabilities are taken relative to, and delta; arrays padded to whole tiles per head, so that they load in bulk.
 // Rows behind the last query and rows without keys get L = +inf: probability 0.
@@ -80,10 +87,11 @@ __global__ void __launch_bounds__(256) row_data_kernel(const Params p, const Row
 template <int DP> struct DkvSmem {
     static constexpr uint32_t kTile = kBox * (DP / 64);
     static constexpr int kStages = DP == 64 ? 4 : 2;
-    static constexpr uint32_t kVec = 3 * kRows * 4;                      // shift, log_sum, delta
-    static constexpr uint32_t kStage = 2 * kTile;                        // Q, dO
+    static constexpr int kSets = DP == 64 ? 2 : 1, kCols = 32 * kSets;         // sets of warps, columns (queries) of a thread
+    static constexpr uint32_t kVec = 3 * kRows * 4;                            // shift, log_sum, delta
+    static constexpr uint32_t kStage = 2 * kTile;                              // Q, dO
     static constexpr uint32_t kRing = 2 * kTile, kVecs = kRing + kStages * kStage, kBars = kVecs + kStages * kVec;
-    static constexpr uint32_t kBytes = kBars + 256 + 1024;
+    static constexpr uint32_t kBytes = kBars + 512 + 1024;
 };
 
 template <int DP, bool kMask>
@@ -96,11 +104,19 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t *gen = raw + (base - smem_u32(raw));
     const uint32_t bars = base + L::kBars;
-    const uint32_t kv_full = bars, s_full = bars + 8, d_full = bars + 16, p_full = bars + 24, ds_full = bars + 32, done = bars + 40;
-    const auto q_full = [&](int s) { return bars + 48u + 8u * s; };
-    const auto g_full = [&](int s) { return bars + 48u + 8u * (L::kStages + s); };
-    const auto empty = [&](int s) { return bars + 48u + 8u * (2 * L::kStages + s); };
-    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + 48 + 24 * L::kStages);
+    const uint32_t kv_full = bars, done = bars + 8;
+    // of the set that takes step x
+    constexpr int kSets = L::kSets, kCols = L::kCols;
+    const auto s_full = [&](int x) { return bars + 16u + 8u * (x % kSets); };
+    const auto d_full = [&](int x) { return bars + 32u + 8u * (x % kSets); };
+    const auto p_full = [&](int x) { return bars + 48u + 8u * (x % kSets); };
+    const auto ds_full = [&](int x) { return bars + 64u + 8u * (x % kSets); };
+    const auto turn = [&](int x) { return (uint32_t)(x / kSets) & 1u; };        // the phase of step x on them
+    const auto q_full = [&](int s) { return bars + 80u + 8u * s; };
+    const auto g_full = [&](int s) { return bars + 80u + 8u * (L::kStages + s); };
+    const auto empty = [&](int s) { return bars + 80u + 8u * (2 * L::kStages + s); };
+    constexpr uint32_t kSlot = 80 + 24 * L::kStages;
+    volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + kSlot);
     int *status = &g_status;
 
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -114,23 +130,28 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     const int per_head = uniform(ie > ib ? ie - ib : 0), steps = per_head * p.group;
 
     if (threadIdx.x == 0) {
-        acp::mbar_init(kv_full, 1); acp::mbar_init(s_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(p_full, 256); acp::mbar_init(ds_full, 256);
-        acp::mbar_init(done, 1);
+        acp::mbar_init(kv_full, 1); acp::mbar_init(done, 1);
+        for (int x = 0; x < kSets; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(d_full(x), 1); acp::mbar_init(p_full(x), 512 / kSets); acp::mbar_init(ds_full(x), 512 / kSets); }
         for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(q_full(s), 1); acp::mbar_init(g_full(s), 1); acp::mbar_init(empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + 48u + 24u * L::kStages) : "memory");
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     fence_before();
     __syncthreads();
     fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t tS = tmem, tD = tmem + 128u, tV = tmem + 256u, tK = tmem + 256u + DP;
+    const auto tS = [&](int x) { return tmem + 128u * (x % kSets); };
+    const uint32_t tD = tmem + 128u * kSets, tV = tmem + 512u - 2 * DP, tK = tmem + 512u - DP;
+    // P over the first columns that a thread read of S; dS over the columns behind them, or over those of dP
+    const auto tG = [&](int x) { return kSets == 2 ? tS(x) + kCols / 2 : tD; };
 
-    if (warp == 9) {
+    if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdRegsLess));
+    if (warp == 17) {
         if (lane == 0 && steps > 0) {
             acp::mbar_expect_tx(kv_full, 2 * L::kTile);
             load_tile<DP>(base, &mk, kv_full, j0, kh, b);
@@ -152,91 +173,83 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 if (++s == L::kStages) { s = 0; ph ^= 1u; }
             }
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         if (steps > 0) {
             const bool one = elect();
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kStage; };
-            const auto phase = [&](int x) { return (uint32_t)(x / L::kStages) & 1u; };
-            bool ok = wait_warp(kv_full, 0u, 22, status) && wait_warp(q_full(0), 0u, 23, status);
-            if (ok) {
+            const auto scores = [&](int x) {                              // S^T = K Q^T
+                if (!wait_warp(q_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, 22, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tS, base, stage(0));                              // S^T = K Q^T
-                    commit(s_full);
+                    product_rows<DP>(tS(x), base, stage(x));
+                    commit(s_full(x));
                 }
                 __syncwarp();
-                ok = wait_warp(g_full(0), 0u, 24, status);
-            }
-            if (ok) {
+                return true;
+            };
+            const auto grads = [&](int x) {                               // dP^T = V dO^T
+                if (!wait_warp(g_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, 23, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tD, base + L::kTile, stage(0) + L::kTile);        // dP^T = V dO^T
-                    commit(d_full);
+                    product_rows<DP>(tD, base + L::kTile, stage(x) + L::kTile);
+                    commit(d_full(x));
                 }
                 __syncwarp();
-            }
+                return true;
+            };
+            bool ok = wait_warp(kv_full, 0u, 24, status);
+            for (int x = 0; x < kSets && x < steps && ok; ++x) ok = scores(x);
+            ok = ok && grads(0);
             for (int x = 0; x < steps && ok; ++x) {
-                ok = wait_warp(p_full, (uint32_t)x & 1u, 25, status);
+                ok = wait_warp(p_full(x), turn(x), 25, status);
                 if (!ok) break;
                 fence_after();
-                if (one) product_cols<DP, kRows, 64>(tV, tS, stage(x) + L::kTile, x != 0);   // dV += P^T dO
+                if (one) product_cols<DP, kRows, kCols>(tV, tS(x), stage(x) + L::kTile, x != 0);      // dV += P^T dO
                 __syncwarp();
-                if (x + 1 < steps) {
-                    ok = wait_warp(q_full((x + 1) % L::kStages), phase(x + 1), 26, status);
-                    if (!ok) break;
-                    fence_after();
-                    if (one) {
-                        product_rows<DP>(tS, base, stage(x + 1));
-                        commit(s_full);
-                    }
-                    __syncwarp();
-                }
-                ok = wait_warp(ds_full, (uint32_t)x & 1u, 27, status);
+                if (kSets == 1 && x + 1 < steps) ok = scores(x + 1);
+                ok = ok && wait_warp(ds_full(x), turn(x), 26, status);
                 if (!ok) break;
                 fence_after();
+                if (kSets == 2 && x + 1 < steps) ok = grads(x + 1);       // dP of this step has been read
+                if (!ok) break;
                 if (one) {
-                    product_cols<DP, kRows, 64>(tK, tD, stage(x), x != 0);                      // dK += dS^T Q
+                    product_cols<DP, kRows, kCols>(tK, tG(x), stage(x), x != 0);                      // dK += dS^T Q
                     commit(empty(x % L::kStages));
                 }
                 __syncwarp();
-                if (x + 1 < steps) {
-                    ok = wait_warp(g_full((x + 1) % L::kStages), phase(x + 1), 28, status);
-                    if (!ok) break;
-                    fence_after();
-                    if (one) {
-                        product_rows<DP>(tD, base + L::kTile, stage(x + 1) + L::kTile);
-                        commit(d_full);
-                    }
-                    __syncwarp();
-                }
+                if (kSets == 1 && x + 1 < steps) ok = grads(x + 1);
+                if (kSets == 2 && x + 2 < steps) ok = scores(x + 2);      // over P and dS of this step
             }
             if (ok && one) commit(done);
         }
-    } else if (warp < 8) {
-        const int half = warp >> 2, row = threadIdx.x & 127, j = j0 + row;
-        const uint32_t mine = ((uint32_t)(warp & 3) << 21) + 64u * half;           // this warp's lanes and columns
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRegsMore));
+        const int set = kSets == 2 ? warp >> 3 : 0, part = kSets == 2 ? (warp >> 2) & 1 : warp >> 2, row = threadIdx.x & 127, j = j0 + row;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, mine = lanes + (uint32_t)(kCols * part);      // this warp's lanes and columns
         const float c = p.scale * kLog2e;
         bool ok = true;
-        for (int x = 0; x < steps; ++x) {
+        for (int x = set; x < steps; x += kSets) {
+            const uint32_t ring = (uint32_t)(x / L::kStages) & 1u;
             const int s = x % L::kStages, h = kh * p.group + x / per_head, i0 = (ib + x % per_head) * kRows;
-            const float *vec = reinterpret_cast<const float *>(gen + L::kVecs + s * L::kVec) + 64 * half;
-            ok = wait(s_full, (uint32_t)x & 1u, 29, status) && wait(q_full(s), (uint32_t)(x / L::kStages) & 1u, 30, status);
+            const float *vec = reinterpret_cast<const float *>(gen + L::kVecs + s * L::kVec) + kCols * part;
+            ok = wait(s_full(x), turn(x), 27, status) && wait(q_full(s), ring, 28, status);
             if (!__all_sync(~0u, ok)) { ok = false; break; }
             fence_after();
-            uint32_t r[64];
-            ld32(tS + mine, r);
-            ld32(tS + mine + 32u, r + 32);
+            uint32_t r[kCols];
+#pragma unroll
+            for (int e = 0; e < kCols; e += 32) ld32(tS(x) + mine + (uint32_t)e, r + e);
             wait_ld();
-            const int first = i0 + 64 * half;                                     // query of column 0 of this half
+            const int first = i0 + kCols * part;                          // query of this thread's column 0
             if (kMask) {
 #pragma unroll
-                for (int e = 0; e < 64; ++e) {
+                for (int e = 0; e < kCols; ++e) {
                     const float y = sees(p, first + e, j, keys) ? masked_score(p, __uint_as_float(r[e]) * p.scale, b, h, first + e, j) : -CUDART_INF_F;
                     r[e] = __float_as_uint(y == -CUDART_INF_F ? 0.0f : ex2(fmaf(y - vec[e], kLog2e, -vec[kRows + e])));
                 }
             } else {
 #pragma unroll
-                for (int e = 0; e < 64; e += 4) {
+                for (int e = 0; e < kCols; e += 4) {
                     const float4 sh = *reinterpret_cast<const float4 *>(vec + e);
                     r[e] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e]), c, -sh.x)));
                     r[e + 1] = __float_as_uint(ex2(fmaf(__uint_as_float(r[e + 1]), c, -sh.y)));
@@ -245,59 +258,62 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 }
                 if ((p.causal && j0 + kRows - 1 > i0 + p.offset) || (p.window && j0 <= i0 + kRows - 1 + p.offset - p.window)) {
                     // columns [lo, hi) see this key
-                    const int lo = p.causal ? j - p.offset - first : 0, hi = p.window ? j - p.offset + p.window - first : 64;
+                    const int lo = p.causal ? j - p.offset - first : 0, hi = p.window ? j - p.offset + p.window - first : kCols;
 #pragma unroll
-                    for (int e = 0; e < 64; ++e)
+                    for (int e = 0; e < kCols; ++e)
                         if (e < lo || e >= hi) r[e] = 0u;
                 }
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < kCols / 16; ++e) {
                 uint32_t y[8];
 #pragma unroll
                 for (int z = 0; z < 8; ++z) y[z] = pack2(__uint_as_float(r[16 * e + 2 * z]), __uint_as_float(r[16 * e + 2 * z + 1]));
-                st8(tS + mine + 8u * e, y);
+                st8(tS(x) + mine + 8u * e, y);
             }
             wait_st();
             fence_before();
-            acp::mbar_arrive(p_full);
-            ok = wait(d_full, (uint32_t)x & 1u, 31, status) && wait(g_full(s), (uint32_t)(x / L::kStages) & 1u, 32, status);
+            acp::mbar_arrive(p_full(x));
+            ok = wait(d_full(x), turn(x), 29, status) && wait(g_full(s), ring, 30, status);
             if (!__all_sync(~0u, ok)) { ok = false; break; }
             fence_after();
-            uint32_t d[64];
-            ld32(tD + mine, d);
-            ld32(tD + mine + 32u, d + 32);
-            wait_ld();
             const float *del = vec + 2 * kRows;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t y[8];
+            for (int n = 0; n < kCols; n += 32) {
+                uint32_t d[32];
+                ld32(tD + mine + (uint32_t)n, d);
+                wait_ld();
 #pragma unroll
-                for (int z = 0; z < 8; z += 2) {
-                    const int a = 16 * e + 2 * z;
-                    const float4 de = *reinterpret_cast<const float4 *>(del + a);
-                    y[z] = pack2(__uint_as_float(r[a]) * (__uint_as_float(d[a]) - de.x), __uint_as_float(r[a + 1]) * (__uint_as_float(d[a + 1]) - de.y));
-                    y[z + 1] = pack2(__uint_as_float(r[a + 2]) * (__uint_as_float(d[a + 2]) - de.z), __uint_as_float(r[a + 3]) * (__uint_as_float(d[a + 3]) - de.w));
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t y[8];
+#pragma unroll
+                    for (int z = 0; z < 8; z += 2) {
+                        const int a = 16 * e + 2 * z;
+                        const float4 de = *reinterpret_cast<const float4 *>(del + n + a);
+                        y[z] = pack2(__uint_as_float(r[n + a]) * (__uint_as_float(d[a]) - de.x), __uint_as_float(r[n + a + 1]) * (__uint_as_float(d[a + 1]) - de.y));
+                        y[z + 1] = pack2(__uint_as_float(r[n + a + 2]) * (__uint_as_float(d[a + 2]) - de.z), __uint_as_float(r[n + a + 3]) * (__uint_as_float(d[a + 3]) - de.w));
+                    }
+                    st8(tG(x) + mine + (uint32_t)(n / 2 + 8 * e), y);
                 }
-                st8(tD + mine + 8u * e, y);
             }
             wait_st();
             fence_before();
-            acp::mbar_arrive(ds_full);
+            acp::mbar_arrive(ds_full(x));
         }
         if (ok && steps > 0) {
-            ok = wait(done, 0u, 33, status);
+            ok = wait(done, 0u, 31, status);
             ok = __all_sync(~0u, ok);
             fence_after();
         }
         if (ok) {
-            // warps 0-3 write dV, warps 4-7 dK; keys behind the length get zeros
-            const uint32_t acc = (half ? tK : tV) + ((uint32_t)(warp & 3) << 21);
-            __nv_bfloat16 *out = half ? static_cast<__nv_bfloat16 *>(p.dk) + b * p.dk_b + kh * p.dk_h + j * p.dk_t
-                                      : static_cast<__nv_bfloat16 *>(p.dv) + b * p.dv_b + kh * p.dv_h + j * p.dv_t;
-            const float f = half ? p.scale : 1.0f;
+            // warps 0-7 write dV, warps 8-15 dK, each half of the columns; keys behind the length get zeros
+            const int key = warp >> 3, side = (warp >> 2) & 1;
+            const uint32_t acc = (key ? tK : tV) + lanes;
+            __nv_bfloat16 *out = key ? static_cast<__nv_bfloat16 *>(p.dk) + b * p.dk_b + kh * p.dk_h + j * p.dk_t
+                                     : static_cast<__nv_bfloat16 *>(p.dv) + b * p.dv_b + kh * p.dv_h + j * p.dv_t;
+            const float f = key ? p.scale : 1.0f;
 #pragma unroll 1
-            for (int x = 0; x < DP / 32; ++x) {
+            for (int x = side * (DP / 64); x < (side + 1) * (DP / 64); ++x) {
                 uint32_t o[32];
                 if (steps > 0) { ld32(acc + 32u * x, o); wait_ld(); }
                 if (steps == 0 || j >= keys) {
@@ -311,7 +327,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     linger_if_failed(status);
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
@@ -322,7 +338,7 @@ template <int DP> struct DqSmem {
     static constexpr uint32_t kTile = kBox * (DP / 64);
     static constexpr int kK = DP == 64 ? 4 : 3, kV = DP == 64 ? 4 : 2;
     static constexpr uint32_t kRingK = 2 * kTile, kRingV = kRingK + kK * kTile, kBars = kRingV + kV * kTile;
-    static constexpr uint32_t kBytes = kBars + 256 + 1024;
+    static constexpr uint32_t kBytes = kBars + 512 + 1024;
 };
 
 template <int DP, bool kMask>
@@ -335,13 +351,16 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     const uint32_t base = (smem_u32(raw) + 1023u) & ~1023u;
     uint8_t *gen = raw + (base - smem_u32(raw));
     const uint32_t bars = base + L::kBars;
-    const uint32_t q_full = bars, g_full = bars + 8, d_full = bars + 16, ds_full = bars + 24, done = bars + 32, fix = bars + 40;
-    const auto s_full = [&](int x) { return bars + 48u + 8u * x; };
-    const auto k_full = [&](int s) { return bars + 64u + 8u * s; };
-    const auto k_empty = [&](int s) { return bars + 64u + 8u * (L::kK + s); };
-    const auto v_full = [&](int s) { return bars + 64u + 8u * (2 * L::kK + s); };
-    const auto v_empty = [&](int s) { return bars + 64u + 8u * (2 * L::kK + L::kV + s); };
-    constexpr uint32_t kSlot = 64 + 16 * (L::kK + L::kV);
+    const uint32_t q_full = bars, g_full = bars + 8, done = bars + 16, fix = bars + 24;
+    // of set x
+    const auto s_full = [&](int x) { return bars + 32u + 8u * (x & 1); };
+    const auto d_full = [&](int x) { return bars + 48u + 8u * (x & 1); };
+    const auto ds_full = [&](int x) { return bars + 64u + 8u * (x & 1); };
+    const auto k_full = [&](int s) { return bars + 80u + 8u * s; };
+    const auto k_empty = [&](int s) { return bars + 80u + 8u * (L::kK + s); };
+    const auto v_full = [&](int s) { return bars + 80u + 8u * (2 * L::kK + s); };
+    const auto v_empty = [&](int s) { return bars + 80u + 8u * (2 * L::kK + L::kV + s); };
+    constexpr uint32_t kSlot = 80 + 16 * (L::kK + L::kV);
     volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + kSlot);
     int *status = &g_status;
 
@@ -355,14 +374,14 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     const int steps = uniform(ke > kb ? ke - kb : 0);
 
     if (threadIdx.x == 0) {
-        acp::mbar_init(q_full, 1); acp::mbar_init(g_full, 1); acp::mbar_init(d_full, 1); acp::mbar_init(ds_full, 256); acp::mbar_init(done, 1);
-        acp::mbar_init(fix, 1); acp::mbar_init(s_full(0), 1); acp::mbar_init(s_full(1), 1);
+        acp::mbar_init(q_full, 1); acp::mbar_init(g_full, 1); acp::mbar_init(done, 1); acp::mbar_init(fix, 1);
+        for (int x = 0; x < 2; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(d_full(x), 1); acp::mbar_init(ds_full(x), 256); }
         for (int s = 0; s < L::kK; ++s) { acp::mbar_init(k_full(s), 1); acp::mbar_init(k_empty(s), 1); }
         for (int s = 0; s < L::kV; ++s) { acp::mbar_init(v_full(s), 1); acp::mbar_init(v_empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -370,9 +389,12 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     __syncthreads();
     fence_after();
     const uint32_t tmem = *slot;
-    const uint32_t tD = tmem + 256u, tQ = tmem + 384u;                     // S: columns 0 and 128 in turn
+    const auto tS = [&](int x) { return tmem + 128u * (x & 1); };
+    const uint32_t tD = tmem + 256u, tQ = tmem + 384u;
 
-    if (warp == 9) {
+    if (warp >= 16) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdRegsLess));
+    if (warp == 17) {
         bool ok = steps > 0;
         if (ok && lane == 0) {
             acp::mbar_expect_tx(q_full, L::kTile);
@@ -414,7 +436,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             }
             __syncwarp();
         }
-    } else if (warp == 8) {
+    } else if (warp == 16) {
         if (steps > 0) {
             const bool one = elect();
             const auto kt = [&](int x) { return base + L::kRingK + (uint32_t)(x % L::kK) * L::kTile; };
@@ -423,8 +445,8 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                 if (!wait_warp(k_full(x % L::kK), (uint32_t)(x / L::kK) & 1u, 24, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tmem + 128u * (x & 1), base, kt(x));
-                    commit(s_full(x & 1));
+                    product_rows<DP>(tS(x), base, kt(x));
+                    commit(s_full(x));
                 }
                 __syncwarp();
                 return true;
@@ -434,7 +456,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                 fence_after();
                 if (one) {
                     product_rows<DP>(tD, base + L::kTile, vt(x));
-                    commit(d_full);
+                    commit(d_full(x));
                     commit(v_empty(x % L::kV));
                 }
                 __syncwarp();
@@ -443,35 +465,39 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             bool ok = wait_warp(q_full, 0u, 26, status) && scores(0) && wait_warp(g_full, 0u, 27, status) && grads(0);
             if (ok && steps > 1) ok = scores(1);
             for (int x = 0; x < steps && ok; ++x) {
-                ok = wait_warp(ds_full, (uint32_t)x & 1u, 28, status);
+                ok = wait_warp(ds_full(x), (uint32_t)(x / 2) & 1u, 28, status);
                 if (!ok) break;
                 fence_after();
+                if (x + 1 < steps) ok = grads(x + 1);                     // dP of this step has been read; before dQ, since the other set waits for it
+                if (!ok) break;
                 if (one) {
-                    product_cols<DP, kRows, 64>(tQ, tD, kt(x), x != 0);                // dQ += dS K
+                    product_cols<DP, kRows, 64>(tQ, tS(x), kt(x), x != 0);                   // dQ += dS K
                     commit(k_empty(x % L::kK));
                 }
                 __syncwarp();
-                if (x + 1 < steps) ok = grads(x + 1);
-                if (ok && x + 2 < steps) ok = scores(x + 2);              // its columns were read before dS of this step was written
+                if (x + 2 < steps) ok = scores(x + 2);                    // over dS of this step, behind the product that reads it
             }
             if (ok && one) commit(done);
         }
-    } else if (warp < 8) {
-        const int half = warp >> 2, row = threadIdx.x & 127, i = i0 + row;
-        const uint32_t mine = ((uint32_t)(warp & 3) << 21) + 64u * half;
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBwdRegsMore));
+        const int set = warp >> 3, part = (warp >> 2) & 1, row = threadIdx.x & 127, i = i0 + row;
+        const uint32_t mine = ((uint32_t)(warp & 3) << 21) + 64u * part;
         const float c = p.scale * kLog2e;
         const long long at = ((long long)b * p.q_heads + h) * w.padded + i;        // padded rows exist
         const float shift = w.shift[at], log_sum = kMask ? w.log_sum[at] : 0.0f, delta = w.delta[at];
         bool ok = true;
-        for (int x = 0; x < steps; ++x) {
-            ok = wait(s_full(x & 1), (uint32_t)(x / 2) & 1u, 29, status);
+        for (int x = set; x < steps; x += 2) {
+            const uint32_t phase = (uint32_t)(x / 2) & 1u;
+            ok = wait(s_full(x), phase, 29, status);
             if (!__all_sync(~0u, ok)) { ok = false; break; }
             fence_after();
             uint32_t r[64];
-            ld32(tmem + 128u * (x & 1) + mine, r);
-            ld32(tmem + 128u * (x & 1) + mine + 32u, r + 32);
+            ld32(tS(x) + mine, r);
+            ld32(tS(x) + mine + 32u, r + 32);
             wait_ld();
-            const int j0 = (kb + x) * kRows, first = j0 + 64 * half;
+            const int j0 = (kb + x) * kRows, first = j0 + 64 * part;
             if (kMask) {
 #pragma unroll
                 for (int e = 0; e < 64; ++e) {
@@ -490,26 +516,29 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                         if (e < lo || e >= hi) r[e] = 0u;
                 }
             }
-            ok = wait(d_full, (uint32_t)x & 1u, 30, status);
+            ok = wait(d_full(x), phase, 30, status);
             if (!__all_sync(~0u, ok)) { ok = false; break; }
             fence_after();
-            uint32_t d[64];
-            ld32(tD + mine, d);
-            ld32(tD + mine + 32u, d + 32);
-            wait_ld();
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t y[8];
+            for (int n = 0; n < 2; ++n) {
+                uint32_t d[32];
+                ld32(tD + mine + 32u * n, d);
+                wait_ld();
 #pragma unroll
-                for (int z = 0; z < 8; ++z) {
-                    const int a = 16 * e + 2 * z;
-                    y[z] = pack2(__uint_as_float(r[a]) * (__uint_as_float(d[a]) - delta), __uint_as_float(r[a + 1]) * (__uint_as_float(d[a + 1]) - delta));
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t y[8];
+#pragma unroll
+                    for (int z = 0; z < 8; ++z) {
+                        const int a = 16 * e + 2 * z;
+                        y[z] = pack2(__uint_as_float(r[32 * n + a]) * (__uint_as_float(d[a]) - delta),
+                                     __uint_as_float(r[32 * n + a + 1]) * (__uint_as_float(d[a + 1]) - delta));
+                    }
+                    st8(tS(x) + mine + 16u * n + 8u * e, y);
                 }
-                st8(tD + mine + 8u * e, y);
             }
             wait_st();
             fence_before();
-            acp::mbar_arrive(ds_full);
+            acp::mbar_arrive(ds_full(x));
         }
         if (ok && steps > 0) {
             ok = wait(done, 0u, 31, status);
@@ -517,24 +546,24 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             fence_after();
         }
         if (ok) {
-            // each half of the warps writes half of the columns
+            // 32 columns for four warps
             __nv_bfloat16 *out = static_cast<__nv_bfloat16 *>(p.dq) + b * p.dq_b + h * p.dq_h + i * p.dq_t;
-#pragma unroll 1
-            for (int x = half * (DP / 64); x < (half + 1) * (DP / 64); ++x) {
+            const int chunk = warp >> 2;
+            if (chunk < DP / 32) {
                 uint32_t o[32];
-                if (steps > 0) { ld32(tQ + ((uint32_t)(warp & 3) << 21) + 32u * x, o); wait_ld(); }
+                if (steps > 0) { ld32(tQ + ((uint32_t)(warp & 3) << 21) + 32u * chunk, o); wait_ld(); }
                 else {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) o[e] = 0u;
                 }
-                if (i < p.q_len) store_piece(out, 32 * x, p.head_size, o, p.scale);
+                if (i < p.q_len) store_piece(out, 32 * chunk, p.head_size, o, p.scale);
             }
         }
     }
     linger_if_failed(status);
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
     }
