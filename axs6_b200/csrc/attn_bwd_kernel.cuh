@@ -129,12 +129,21 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     const int ie = j0 < keys ? (end_query(p, j1) + kRows - 1) / kRows : 0;
     const int per_head = uniform(ie > ib ? ie - ib : 0), steps = per_head * p.group;
 
-    if (threadIdx.x == 0) {
+    // the thread that issues the loads sets the barriers up and sends the first loads off before the others are ready
+    if (threadIdx.x == 544) {
+        failed() = 0;
         acp::mbar_init(kv_full, 1); acp::mbar_init(done, 1);
         for (int x = 0; x < kSets; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(d_full(x), 1); acp::mbar_init(p_full(x), 512 / kSets); acp::mbar_init(ds_full(x), 512 / kSets); }
         for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(q_full(s), 1); acp::mbar_init(g_full(s), 1); acp::mbar_init(empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
+        if (steps > 0) {
+            acp::mbar_expect_tx(kv_full, 2 * L::kTile);
+            load_tile<DP>(base, &mk, kv_full, j0, kh, b);
+            load_tile<DP>(base + L::kTile, &mv, kv_full, j0, kh, b);
+            prefetch_map(&mq);
+            prefetch_map(&mg);
+        }
     }
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
@@ -153,9 +162,6 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdRegsLess));
     if (warp == 17) {
         if (lane == 0 && steps > 0) {
-            acp::mbar_expect_tx(kv_full, 2 * L::kTile);
-            load_tile<DP>(base, &mk, kv_full, j0, kh, b);
-            load_tile<DP>(base + L::kTile, &mv, kv_full, j0, kh, b);
             int s = 0;
             uint32_t ph = 0;
             for (int x = 0; x < steps; ++x) {
@@ -324,9 +330,9 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
             }
         }
     }
-    linger_if_failed(status);
     fence_before();
     __syncthreads();
+    linger_if_failed();
     if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
@@ -373,13 +379,23 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     const int ke = (end_key(p, i0 + kRows < p.q_len ? i0 + kRows : p.q_len, keys) + kRows - 1) / kRows;
     const int steps = uniform(ke > kb ? ke - kb : 0);
 
-    if (threadIdx.x == 0) {
+    // the thread that issues the loads sets the barriers up and sends the first loads off before the others are ready
+    if (threadIdx.x == 544) {
+        failed() = 0;
         acp::mbar_init(q_full, 1); acp::mbar_init(g_full, 1); acp::mbar_init(done, 1); acp::mbar_init(fix, 1);
         for (int x = 0; x < 2; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(d_full(x), 1); acp::mbar_init(ds_full(x), 256); }
         for (int s = 0; s < L::kK; ++s) { acp::mbar_init(k_full(s), 1); acp::mbar_init(k_empty(s), 1); }
         for (int s = 0; s < L::kV; ++s) { acp::mbar_init(v_full(s), 1); acp::mbar_init(v_empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
+        if (steps > 0) {
+            acp::mbar_expect_tx(q_full, L::kTile);
+            load_tile<DP>(base, &mq, q_full, i0, h, b);
+            acp::mbar_expect_tx(g_full, L::kTile);
+            load_tile<DP>(base + L::kTile, &mg, g_full, i0, h, b);
+            prefetch_map(&mk);
+            prefetch_map(&mv);
+        }
     }
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
@@ -395,13 +411,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBwdRegsLess));
     if (warp == 17) {
-        bool ok = steps > 0;
-        if (ok && lane == 0) {
-            acp::mbar_expect_tx(q_full, L::kTile);
-            load_tile<DP>(base, &mq, q_full, i0, h, b);
-            acp::mbar_expect_tx(g_full, L::kTile);
-            load_tile<DP>(base + L::kTile, &mg, g_full, i0, h, b);
-        }
+        bool ok = true;
         for (int x = 0; x < steps && ok; ++x) {
             const int row = (kb + x) * kRows, ks = x % L::kK, vs = x % L::kV;
             const uint32_t kd = base + L::kRingK + ks * L::kTile, vd = base + L::kRingV + vs * L::kTile;
@@ -560,9 +570,9 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             }
         }
     }
-    linger_if_failed(status);
     fence_before();
     __syncthreads();
+    linger_if_failed();
     if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

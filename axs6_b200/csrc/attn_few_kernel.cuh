@@ -59,12 +59,19 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     const int steps = uniform(to > from ? to - from : 0);
     if (steps == 0 && chunk > 0) return;                                   // the join does not read this chunk
 
-    if (threadIdx.x == 0) {
+    // the thread that issues the loads sets the barriers up and sends the first loads off before the others are ready
+    if (threadIdx.x == 160) {
+        failed() = 0;
         acp::mbar_init(q_full, 128); acp::mbar_init(o_full, 1); acp::mbar_init(fix, 1);
         for (int x = 0; x < 2; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(o_done(x), 1); acp::mbar_init(p_full(x), (uint32_t)(r1 - r0 + 31) / 32u * 32u); }
         for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(kv_full(s), 1); acp::mbar_init(kv_empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
+        if (steps > 0) {
+            acp::mbar_expect_tx(kv_full(0), L::kTile);
+            load_tile<DP, kKeys>(base + L::kRing, &mk, kv_full(0), from * kKeys, kh, b);
+            prefetch_map(&mv);
+        }
     }
     if (warp == 4) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 256;" ::"r"(bars + 72u + 16u * L::kStages) : "memory");
@@ -77,9 +84,9 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
 
     if (warp == 5) {
         bool ok = true;
-        int s = 0;
+        int s = 1;                                                        // K of the first tile is under way
         uint32_t ph = 0;
-        for (int x = 0; x < 2 * steps && ok; ++x) {
+        for (int x = 1; x < 2 * steps && ok; ++x) {
             const int row = (from + x / 2) * kKeys;
             ok = wait_warp(kv_empty(s), ph ^ 1u, 1, status);
             if (!ok) break;
@@ -249,9 +256,9 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
             }
         }
     }
-    linger_if_failed(status);
     fence_before();
     __syncthreads();
+    linger_if_failed();
     if (warp == 4) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 256;" ::"r"(tmem));

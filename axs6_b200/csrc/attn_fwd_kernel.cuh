@@ -76,13 +76,25 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     // Units in the order of their products: both tiles of each step, then what the longer walk has left.
     const auto unit_of = [&](int j, int t) { return j < both ? 2 * j + t : both + j; };
 
-    if (threadIdx.x == 0) {
+    // the thread that issues the loads sets the barriers up and sends the first loads off before the others are ready
+    if (threadIdx.x == 544) {
+        failed() = 0;
         for (int t = 0; t < 2; ++t) { acp::mbar_init(q_full(t), 1); acp::mbar_init(o_full(t), 1); acp::mbar_init(o_done(t, 0), 1); acp::mbar_init(o_done(t, 1), 1); }
         for (int x = 0; x < kBufs; ++x) { acp::mbar_init(s_full(x), 1); acp::mbar_init(p_full(x), 256); }
         acp::mbar_init(fix, 1);
         for (int s = 0; s < L::kStages; ++s) { acp::mbar_init(kv_full(s), 1); acp::mbar_init(kv_empty(s), 1); }
         acp::fence_barrier_init();
         acp::fence_async_smem();
+        if (steps > 0) {
+            for (int t = 0; t < 2; ++t)
+                if ((t ? n1 : n0) > 0) {
+                    acp::mbar_expect_tx(q_full(t), L::kTile);
+                    load_tile<DP>(base + t * L::kTile, &mq, q_full(t), i0 + t * kRows, h, b);
+                }
+            acp::mbar_expect_tx(kv_full(0), L::kTile);
+            load_tile<DP>(base + L::kRing, &mk, kv_full(0), kb * kRows, kh, b);
+            prefetch_map(&mv);
+        }
     }
     if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(bars + kSlot) : "memory");
@@ -98,17 +110,11 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     if (warp >= 16) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsLess));
     if (warp == 17) {
-        // ------------------------------------------------------------------ loads: Q, then K_j, V_j in turn
-        bool ok = steps > 0;
-        if (ok && lane == 0)
-            for (int t = 0; t < 2; ++t)
-                if ((t ? n1 : n0) > 0) {
-                    acp::mbar_expect_tx(q_full(t), L::kTile);
-                    load_tile<DP>(base + t * L::kTile, &mq, q_full(t), i0 + t * kRows, h, b);
-                }
-        int s = 0;
+        // ------------------------------------------------------------------ loads: V_0 (Q and K_0 are under way), then K_j, V_j in turn
+        bool ok = true;
+        int s = 1;
         uint32_t ph = 0;
-        for (int x = 0; x < 2 * steps && ok; ++x) {
+        for (int x = 1; x < 2 * steps && ok; ++x) {
             const int row = (kb + x / 2) * kRows;
             ok = wait_warp(kv_empty(s), ph ^ 1u, 1, status);
             if (!ok) break;
@@ -276,9 +282,9 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
             }
         }
     }
-    linger_if_failed(status);
     fence_before();
     __syncthreads();
+    linger_if_failed();
     if (warp == 16) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));

@@ -23,7 +23,13 @@ constexpr uint32_t kWaitPolls = 1u << 20;        // of about a microsecond each,
 
 static __device__ int g_status;                  // 0, or the code of the first wait that gave up (one translation unit includes this)
 
-// false: gave up, or somebody else did.
+// Whether a wait of this CTA gave up
+__device__ __forceinline__ int &failed()
+{
+    __shared__ int f;
+    return f;
+}
+// false: gave up, or somebody else did
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code, int *status)
 {
     for (uint32_t i = 0; i < kWaitPolls; ++i) {
@@ -31,9 +37,10 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, int code, in
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
                      : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
         if (ok) return true;
-        if ((i & 63u) == 63u && *(volatile int *)status != 0) return false;
+        if ((i & 63u) == 63u && *(volatile int *)status != 0) break;
     }
     atomicCAS(status, 0, code);
+    *(volatile int *)&failed() = 1;
     return false;
 }
 
@@ -259,13 +266,14 @@ __device__ __forceinline__ void store_rest(__nv_bfloat16 *row, int c0, int d, ui
     store_piece(row, c0, d, r, 1.0f);
 }
 
-// On the way out of a kernel in which a wait gave up: loads and products that were issued may still be running; they complete within
-// microseconds, so every thread lingers before shared and tensor memory are released.
-__device__ __forceinline__ void linger_if_failed(int *status)
+// On the way out, behind the last barrier: where a wait gave up, loads and products that were issued may still be running; they complete
+// within microseconds, so every thread lingers before shared and tensor memory are released.
+__device__ __forceinline__ void linger_if_failed()
 {
-    if (*(volatile int *)status != 0)
+    if (*(volatile int *)&failed() != 0)
         for (int i = 0; i < 200; ++i) __nanosleep(1000);
 }
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---------------------------------------------------------------------------------------------- host
 // (value, token, head, batch) map of a bf16 tensor, boxes of 64 values x `rows` tokens
