@@ -13,7 +13,9 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..core import DEFAULT_BLOCK_SIZE
+from .attention_unified import axs_attention_unified
 from .functional_unified import axs_linear_unified, fake_quantize_unified
+from .rotary_unified import RotaryFrequencies, axs_rotary_unified
 
 
 class AXSLinearUnified(nn.Module):
@@ -110,11 +112,20 @@ class AXSEmbeddingUnified(nn.Module):
 class AXSMultiheadAttentionUnified(nn.Module):
     """Batch-first multi-head attention: q/k/v/out projections are :class:`AXSLinearUnified`, the scores
     and the softmax stay in full precision, and the attention weights are fake-quantised with stochastic
-    rounding (blocks along the key dimension) before they multiply the values."""
+    rounding (blocks along the key dimension) before they multiply the values.
+
+    ``quantize_weights=False`` leaves the weights unquantised and computes them with
+    :func:`~axs6_b200.unified.attention_unified.axs_attention_unified`, which never writes them to memory (heads of up to 128
+    values, no dropout); ``causal`` and ``key_lengths`` of the call are open to it alone.  ``rotary`` (a plan from ``rotary_frequencies``)
+    rotates the query and key heads by ``positions``, by default 0, 1, ...; ``rotary_layout`` as in ``axs_rotary_unified``."""
 
     def __init__(self, embed_dim: int, num_heads: int, dropout: float = 0.0, bias: bool = True,
-                 block_size: int = DEFAULT_BLOCK_SIZE) -> None:
+                 block_size: int = DEFAULT_BLOCK_SIZE, quantize_weights: bool = True, rotary: RotaryFrequencies | None = None,
+                 rotary_layout: str = "half") -> None:
         super().__init__()
+        if not quantize_weights and dropout > 0:
+            raise ValueError("attention without materialised weights has no dropout")
+        self.quantize_weights, self.rotary, self.rotary_layout = quantize_weights, rotary, rotary_layout
         assert embed_dim % num_heads == 0, "embed_dim must be divisible by num_heads"
         self.embed_dim, self.num_heads, self.head_dim = embed_dim, num_heads, embed_dim // num_heads
         self.block_size, self.dropout = block_size, dropout
@@ -126,8 +137,30 @@ class AXSMultiheadAttentionUnified(nn.Module):
         return t.reshape(t.shape[0], t.shape[1], self.num_heads, self.head_dim).transpose(1, 2)
 
     def forward(self, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
-                attn_mask: torch.Tensor | None = None) -> torch.Tensor:
+                attn_mask: torch.Tensor | None = None, causal: bool = False, key_lengths: torch.Tensor | None = None,
+                positions: torch.Tensor | None = None) -> torch.Tensor:
+        if self.quantize_weights and (causal or key_lengths is not None):
+            raise ValueError("causal and key_lengths need quantize_weights=False; pass attn_mask instead")
+        if positions is not None and self.rotary is None:
+            raise ValueError("positions need a rotary plan")
         q, k, v = self._heads(self.q_proj(query)), self._heads(self.k_proj(key)), self._heads(self.v_proj(value))
+        if self.rotary is not None:
+            plan = self.rotary if self.rotary.turns.device == q.device else self.rotary.to(q.device)
+            self.rotary = plan
+            if positions is None:
+                if query.shape[1] != key.shape[1]:
+                    raise ValueError("positions are needed where queries and keys differ in number")
+                positions = torch.arange(query.shape[1], device=q.device)
+            if query.shape[1] == key.shape[1]:
+                q, k = axs_rotary_unified(q, k, positions, plan, self.rotary_layout)
+            else:                       # positions belong to the keys; the queries are the last of them
+                q, _ = axs_rotary_unified(q, None, positions[..., -query.shape[1]:], plan, self.rotary_layout)
+                _, k = axs_rotary_unified(None, k, positions, plan, self.rotary_layout)
+        if not self.quantize_weights:
+            if attn_mask is not None and attn_mask.is_floating_point() and attn_mask.dtype != torch.bfloat16:
+                attn_mask = attn_mask.float()
+            ctx = axs_attention_unified(q, k, v, causal=causal, key_lengths=key_lengths, mask=attn_mask, scale=self.scale)
+            return self.out_proj(ctx.transpose(1, 2).reshape(query.shape[0], query.shape[1], self.embed_dim))
         scores = torch.matmul(q, k.transpose(-2, -1)) * self.scale
         if attn_mask is not None:
             scores = scores + attn_mask

@@ -148,6 +148,13 @@ class AXSTrainingPipelineUnified:
         return {"loss": float(loss.detach()), "loss_scale": self.loss_scale, "grad_norm": norm, "overflow": False,
                 "step": self._total_steps, "warmup": warmup, "lr": self._current_lr()}
 
+    def distillation_step(self, inputs: Any, teacher: Callable[..., Any], temperature: float = 1.0,
+                          reduction: str = "mean") -> dict[str, Any]:
+        """``training_step`` with the distillation loss: ``teacher(inputs) -> (top logits, their indices)``, one row of slots per
+        position of the model's logits (see ``axs_distillation_unified``)."""
+        from .distillation_unified import AXSDistillationLoss
+        return self.training_step(inputs, AXSDistillationLoss(teacher, temperature, reduction))
+
     # ------------------------------------------------------------------ checkpoints
     def save_checkpoint(self, path, *, extra: dict[str, Any] | None = None) -> Path:
         path = Path(path)
