@@ -74,7 +74,7 @@ SIGNATURES = {
     "axs6_rotary": (_int, [_ptr, _ptr, _i64, _ptr, _ptr, _ptr, _ptr, _i64, _ptr, _ptr, _int, _i64, _i64, _i64, _i64,
                            _ptr, _int, _i64, _i64, _ptr, ctypes.c_float, _int, _int, _ptr]),
     "axs6_distill_fwd": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _int, _i64, _ptr, _i64, _i64, ctypes.c_float, _int,
-                                _ptr, _ptr, _ptr, _ptr]),
+                                _ptr, _ptr, _ptr, _ptr, _ptr]),
     "axs6_distill_bwd": (_int, [_ptr, _int, _i64, _i64, _i64, _ptr, _int, _i64, _ptr, _i64, _i64, ctypes.c_float,
                                 _ptr, _ptr, _i64, _ptr, _ptr, _i64, _ptr]),
     "axs6_attn_fwd": (_int, [ctypes.POINTER(AttnArgs), _ptr]),

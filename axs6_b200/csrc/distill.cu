@@ -266,8 +266,8 @@ __global__ void __launch_bounds__(kThreads, 4) forward_kernel(const Params p)
     }
 }
 
-// Sum of the rows' losses, or their mean over the rows with a used slot, in 64 bits and in a fixed order; out[1] = that number of rows.
-__global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, const float4 *stats, long long rows, int mean, float *out)
+// Sum of the rows' losses, or their mean over the rows with a used slot, in 64 bits and in a fixed order; *count = that number of rows, at least 1.
+__global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, const float4 *stats, long long rows, int mean, float *out, float *count)
 {
     __shared__ double sum_s[32];
     __shared__ long long cnt_s[32];
@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(1024) reduce_kernel(const float *row_loss, con
         for (int o = 16; o; o >>= 1) { sum += __shfl_xor_sync(~0u, sum, o); cnt += __shfl_xor_sync(~0u, cnt, o); }
         if (threadIdx.x == 0) {
             const double n = cnt ? (double)cnt : 1.0;
-            out[0] = (float)(mean ? sum / n : sum);
-            out[1] = (float)n;
+            *out = (float)(mean ? sum / n : sum);
+            *count = (float)n;
         }
     }
 }
@@ -410,12 +410,12 @@ static int segments_of(const DeviceInfo &d, int64_t rows, int64_t vocab, int esi
 
 AXS6_API int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
                               int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature, int reduction,
-                              float *row_loss, float *row_stats, float *reduced, axs6_stream_t stream)
+                              float *row_loss, float *row_stats, float *reduced, float *count, axs6_stream_t stream)
 {
     using namespace axs6;
     using namespace axs6::distill;
     if (!args_ok(logits, dtype, rows, vocab, ld, teacher, teacher_dtype, ld_teacher, index, ld_index, slots, temperature) || reduction < 0 ||
-        reduction > 2 || (rows && (!row_loss || !row_stats)) || (reduction && !reduced))
+        reduction > 2 || (rows && (!row_loss || !row_stats)) || (reduction && (!reduced || !count)))
         return AXS6_ERR_ARG;
     if (slots > kMaxSlots) return AXS6_ERR_UNSUPPORTED;
     if (!aligned16(row_stats)) return AXS6_ERR_ALIGN;
@@ -452,7 +452,7 @@ AXS6_API int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64
         if (rc != AXS6_OK) return rc;
     }
     if (reduction) {
-        if (launch_overlapped(true, reduce_kernel, 1, 1024, 0, st, row_loss, p.stats, (long long)rows, reduction == 2, reduced) != cudaSuccess)
+        if (launch_overlapped(true, reduce_kernel, 1, 1024, 0, st, row_loss, p.stats, (long long)rows, reduction == 2, reduced, count) != cudaSuccess)
             return AXS6_ERR_LAUNCH;
         count_launch();
     }

@@ -5,6 +5,9 @@ CUDA tensors (fp32 or bf16); a CPU tensor raises ``RuntimeError`` -- there is no
 """
 from __future__ import annotations
 
+import ctypes
+from array import array
+
 import torch
 
 from . import _lib
@@ -100,7 +103,9 @@ def _as_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int]:
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    if dev.index is None:
+        return torch.cuda.current_stream(dev).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(dev.index)          # the same handle without a Stream object around it
 
 
 class _on:
@@ -730,28 +735,30 @@ def _heads_view(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
-def _strides3(t: torch.Tensor):
-    import ctypes
-    return (ctypes.c_int64 * 3)(*t.stride()[:3])
-
-
 def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor, turns: torch.Tensor, gain: float = 1.0,
            interleaved: bool = False, inverse: bool = False, who: str = "rotary"):
     """Rotated copies of ``q`` and ``k`` (batch, heads, tokens, size; either may be None) in one launch.  ``turns``: int64 bits of
     each pair's fraction of a turn per position; ``inverse`` turns the other way (the gradient)."""
-    given = [t for t in (q, k) if t is not None]
-    if not given:
+    ref = k if q is None else q
+    if ref is None:
         raise ValueError(f"{who} needs q or k")
-    for t in given:
+    for t in (q, k):
+        if t is None:
+            continue
         _check_input(t, who)
         if t.dim() != 4:
             raise ValueError(f"{who} takes tensors of (batch, heads, tokens, size), got {tuple(t.shape)}")
         if t.dtype not in _DT:
             raise TypeError(f"{who} takes fp32 or bf16 tensors, got {t.dtype}")
-    ref = given[0]
+    dev, dtype = ref.device, ref.dtype
     batch, _, tokens, size = ref.shape
-    if k is not None and q is not None and (k.shape[0], k.shape[2], k.shape[3]) != (batch, tokens, size):
-        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or size")
+    if k is not None and q is not None:
+        if (k.shape[0], k.shape[2], k.shape[3]) != (batch, tokens, size):
+            raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} differ in batch, tokens or size")
+        if k.dtype != dtype:
+            raise ValueError(f"{who}: q and k differ in type")
+        if k.device != dev:
+            raise ValueError(f"{who}: tensors on different devices")
     rotated = 2 * turns.numel()
     if rotated > size:
         raise ValueError(f"{who}: {rotated} values to rotate in heads of {size}")
@@ -760,25 +767,34 @@ def rotary(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tens
                          f"{positions.dtype} {tuple(positions.shape)}")
     if turns.dtype != torch.int64 or turns.dim() != 1:
         raise ValueError(f"{who}: turns must be a 1-D int64 tensor")
-    if any(t.dtype != ref.dtype for t in given):
-        raise ValueError(f"{who}: q and k differ in type")
-    if any(t.device != ref.device for t in (*given, positions, turns)):
+    if positions.device != dev or turns.device != dev:
         raise ValueError(f"{who}: tensors on different devices")
-    turns = turns.contiguous()
-    x = [None if t is None else _heads_view(t) for t in (q, k)]
-    y = [None if t is None else torch.empty_like(t) for t in x]
-    if any(t is not None and t.stride(-1) != 1 and t.shape[-1] > 1 for t in y):
-        y = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in x]
+    if not turns.is_contiguous():
+        turns = turns.contiguous()
 
-    def side(a, b):
-        return (None, None, 0, None, None) if a is None else (a.data_ptr(), b.data_ptr(), a.shape[1], _strides3(a), _strides3(b))
+    out, args, keep = [], [], []
+    for t in (q, k):
+        if t is None:
+            out.append(None)
+            args += (None, None, 0, None, None)
+            continue
+        x = _heads_view(t)
+        y = torch.empty_like(x)
+        if y.stride(3) != 1 and size > 1:
+            y = torch.empty(x.shape, dtype=dtype, device=dev)
+        out.append(y)
+        strides = array("q", x.stride()[:3] + y.stride()[:3])
+        at = strides.buffer_info()[0]
+        keep += (x, strides)
+        args += (x.data_ptr(), y.data_ptr(), x.shape[1], at, at + 24)
     pb, pt = (0, positions.stride(0)) if positions.dim() == 1 else positions.stride()
-    with _on(ref.device):
-        st = _lib.load().axs6_rotary(*side(x[0], y[0]), *side(x[1], y[1]), _DT[ref.dtype], batch, tokens, size, rotated,
-                                     positions.data_ptr(), int(positions.dtype == torch.int64), pb, pt, turns.data_ptr(),
-                                     float(gain), int(interleaved), int(inverse), _stream(ref.device))
-    _lib.check("axs6_rotary", st)
-    return y[0], y[1]
+    with _on(dev):
+        st = _lib.load().axs6_rotary(*args, _DT[dtype], batch, tokens, size, rotated, positions.data_ptr(), positions.dtype == torch.int64,
+                                     pb, pt, turns.data_ptr(), gain, interleaved, inverse, _stream(dev))
+    if st:
+        _lib.check("axs6_rotary", st)
+    del keep
+    return out[0], out[1]
 
 
 # ------------------------------------------------------------------------------------ distillation
@@ -801,22 +817,25 @@ def distill_fwd(logits: torch.Tensor, teacher: torch.Tensor, index: torch.Tensor
         raise ValueError(f"{who}: empty vocabulary")
     if teacher.device != logits.device or index.device != logits.device:
         raise ValueError(f"{who}: tensors on different devices")
-    z, rows, vocab, ldz = _as_rows(logits.detach())
-    t, _, slots, ldt = _as_rows(teacher.detach())
-    ix = index.reshape(-1, slots).to(torch.int64)
+    z, rows, vocab, ldz = _as_rows(logits)
+    t, _, slots, ldt = _as_rows(teacher)
+    ix = index if index.dim() == 2 else index.reshape(-1, slots)
+    if ix.dtype != torch.int64:
+        ix = ix.to(torch.int64)
     if ix.stride(1) != 1 and slots > 1:
         ix = ix.contiguous()
     dev = logits.device
-    row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
+    # the result is a tensor of its own, not a view: autograd lets a caller change it in place
+    row_loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
     stats = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-    reduced = torch.empty(2, dtype=torch.float32, device=dev) if reduction else None
+    loss = torch.empty((), dtype=torch.float32, device=dev) if reduction else row_loss
+    count = torch.empty((), dtype=torch.float32, device=dev) if reduction else None
     with _on(dev):
         st = _lib.load().axs6_distill_fwd(z.data_ptr(), _DT[z.dtype], rows, vocab, ldz, t.data_ptr(), _DT[t.dtype], ldt, ix.data_ptr(),
                                           ix.stride(0), slots, temperature, reduction, row_loss.data_ptr(), stats.data_ptr(),
-                                          reduced.data_ptr() if reduced is not None else None, _stream(dev))
+                                          loss.data_ptr() if reduction else None, count.data_ptr() if reduction else None, _stream(dev))
     _lib.check("axs6_distill_fwd", st)
-    loss = row_loss.reshape(logits.shape[:-1]) if reduced is None else reduced[0]
-    return loss, z, t, ix, stats, reduced[1:] if reduction == 2 else None
+    return loss, z, t, ix, stats, count if reduction == 2 else None
 
 
 def distill_bwd(z: torch.Tensor, t: torch.Tensor, ix: torch.Tensor, stats: torch.Tensor, upstream: torch.Tensor,
@@ -837,37 +856,41 @@ def distill_bwd(z: torch.Tensor, t: torch.Tensor, ix: torch.Tensor, stats: torch
 
 
 # --------------------------------------------------------------------------------------- attention
+def _attn_operand_ok(t: torch.Tensor) -> bool:
+    (n0, n1, n2, size), (s0, s1, s2, s3) = t.shape, t.stride()
+    if s3 != 1 and size != 1:
+        return False
+    return t.dtype == torch.float32 or (t.data_ptr() % 16 == 0 and (n0 == 1 or (s0 % 8 == 0 and s0 > 0))
+                                        and (n1 == 1 or (s1 % 8 == 0 and s1 > 0)) and (n2 == 1 or (s2 % 8 == 0 and s2 > 0)))
+
+
 def _attn_operand(t: torch.Tensor) -> torch.Tensor:
     """A tensor the kernels can read: values adjacent and, for bf16, 16-byte aligned rows and no overlapping ones; a padded
     copy otherwise."""
-    if t.numel() == 0:
+    if t.numel() == 0 or _attn_operand_ok(t):
         return t
     if t.dtype == torch.float32:
-        return _heads_view(t)
-    ok = (t.stride(-1) == 1 or t.shape[-1] == 1) and t.data_ptr() % 16 == 0
-    if ok and all(n == 1 or (s % 8 == 0 and s > 0) for n, s in zip(t.shape[:3], t.stride()[:3])):
-        return t
-    size = t.shape[-1]
+        return t.contiguous()
+    size = t.shape[3]
     buf = torch.empty((*t.shape[:3], _r8(size)), dtype=t.dtype, device=t.device)[..., :size]
     return buf.copy_(t)
 
 
-def _attn_strides(t: torch.Tensor):
-    """Strides {batch, head, token}; those of extents of one, which mean nothing, as if the tensor were packed."""
-    s = list(t.stride()[:3])
-    pitch = _r8(t.shape[3])
-    for d in (2, 1, 0):
-        if t.shape[d] == 1:
-            s[d] = pitch
-        pitch = max(pitch, s[d] * t.shape[d])
-    return s
+def _attn_result(like: torch.Tensor) -> torch.Tensor:
+    """A tensor shaped and, where the kernels can write that, laid out like ``like``; not a view of a larger one."""
+    t = torch.empty_like(like)
+    if t.numel() == 0 or _attn_operand_ok(t):
+        return t
+    _, h, n, size = t.shape
+    pitch = _r8(size)
+    return torch.empty_strided(t.shape, (h * n * pitch, n * pitch, pitch, 1), dtype=t.dtype, device=t.device)
 
 
 def _attn_args(tensors: dict, stats, lse, low, key_lengths, mask, scale: float, causal: bool, window: int) -> "_lib.AttnArgs":
     a = _lib.AttnArgs()
-    for name, t in tensors.items():
+    for name, t in tensors.items():                # strides of extents of one mean nothing and are not used
         setattr(a, name, t.data_ptr())
-        getattr(a, name + "_strides")[:] = _attn_strides(t)
+        getattr(a, name + "_strides")[:] = t.stride()[:3]
     q, k = tensors["q"], tensors["k"]
     a.row_max, a.row_sum = stats[0].data_ptr(), stats[1].data_ptr()
     a.lse = lse.data_ptr() if lse is not None else None
@@ -884,7 +907,6 @@ def _attn_args(tensors: dict, stats, lse, low, key_lengths, mask, scale: float, 
 
 
 def _attn_workspace(a, backward: int, dev):
-    import ctypes
     n = int(_lib.load().axs6_attn_workspace_bytes(ctypes.byref(a), backward))
     if not n:
         return None
@@ -931,12 +953,9 @@ def attention_check(q, k, v, key_lengths, mask, scale, causal, window, who: str)
 def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window: int, want_lse: bool, for_backward: bool = True):
     """-> (o shaped and laid out like q, row statistics (2, batch, heads, queries), lse or None, the operands as read, what rounding
     left of o: bf16 with ``for_backward``, else None)."""
-    import ctypes
     q, k, v = (_attn_operand(t) for t in (q, k, v))
     dev = q.device
-    o = torch.empty_like(q)
-    if o.numel() and _attn_operand(o) is not o:
-        o = torch.empty((*q.shape[:3], _r8(q.shape[3])), dtype=q.dtype, device=dev)[..., :q.shape[3]]
+    o = _attn_result(q)
     stats = torch.empty((2, *q.shape[:3]), dtype=torch.float32, device=dev)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=dev) if want_lse else None
     key_lengths = key_lengths.contiguous() if key_lengths is not None else None
@@ -952,15 +971,11 @@ def attention_fwd(q, k, v, key_lengths, mask, scale: float, causal: bool, window
 
 def attention_bwd(d_o, q, k, v, o, low, stats, key_lengths, mask, scale: float, causal: bool, window: int):
     """-> (dq, dk, dv), each laid out like the tensor it belongs to."""
-    import ctypes
     dev = q.device
     d_o = _attn_operand(d_o)
     grads = []
     for t in (q, k, v):
-        g = torch.empty_like(t)
-        if g.numel() and _attn_operand(g) is not g:
-            g = torch.empty((*t.shape[:3], _r8(t.shape[3])), dtype=t.dtype, device=dev)[..., :t.shape[3]]
-        grads.append(g)
+        grads.append(_attn_result(t))
     key_lengths = key_lengths.contiguous() if key_lengths is not None else None
     a = _attn_args({"q": q, "k": k, "v": v, "o": o, "d_o": d_o, "dq": grads[0], "dk": grads[1], "dv": grads[2]}, stats, None,
                    low, key_lengths, mask, scale, causal, window)

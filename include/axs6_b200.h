@@ -401,13 +401,13 @@ int axs6_rotary(const void *q, void *q_out, int64_t q_heads, const int64_t *q_st
  * [0, vocab) or its logit is -inf; a row without a used slot has loss 0 and is not counted.  1 <= slots <= 1024
  * (AXS6_ERR_UNSUPPORTED above).  row_loss: rows floats, row_stats: 4 * rows floats for the backward call, 16-byte
  * aligned (AXS6_ERR_ALIGN otherwise).  reduction 0: none,
- * 1: reduced[0] = sum, 2: reduced[0] = mean over the counted rows; reduced[1] = their number, at least 1. */
+ * 1: *reduced = sum, 2: *reduced = mean over the counted rows; *count = their number, at least 1. */
 int axs6_distill_fwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
                      int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature, int reduction,
-                     float *row_loss, float *row_stats, float *reduced, axs6_stream_t stream);
+                     float *row_loss, float *row_stats, float *reduced, float *count, axs6_stream_t stream);
 
 /* grad (rows, vocab), in the logits' type, = d (sum over rows of upstream[r * upstream_stride] * row_loss[r]) / d logits, divided by
- * *count if that is not NULL (reduced[1] of a mean).  Slots that name the same index are added in slot order: no atomics. */
+ * *count if that is not NULL (of a mean).  Slots that name the same index are added in slot order: no atomics. */
 int axs6_distill_bwd(const void *logits, int dtype, int64_t rows, int64_t vocab, int64_t ld, const void *teacher, int teacher_dtype,
                      int64_t ld_teacher, const int64_t *index, int64_t ld_index, int64_t slots, float temperature,
                      const float *row_stats, const float *upstream, int64_t upstream_stride, const float *count, void *grad,

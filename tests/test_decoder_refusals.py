@@ -29,9 +29,9 @@ def test_rotary_arguments():
 
 def test_distillation_arguments():
     lib = _lib.load()
-    fwd = dict(z=16, dt=0, rows=2, vocab=10, ld=10, t=16, tdt=0, ldt=3, ix=16, ldi=3, slots=3, temp=1.0, red=2, loss=16, stats=16, out=16)
+    fwd = dict(z=16, dt=0, rows=2, vocab=10, ld=10, t=16, tdt=0, ldt=3, ix=16, ldi=3, slots=3, temp=1.0, red=2, loss=16, stats=16, out=16, cnt=16)
     for bad in (dict(z=None), dict(t=None), dict(ix=None), dict(dt=2), dict(tdt=-1), dict(rows=-1), dict(vocab=0), dict(vocab=1 << 31), dict(slots=0), dict(temp=0.0),
-                dict(temp=float("inf")), dict(temp=float("nan")), dict(red=3), dict(loss=None), dict(stats=None), dict(out=None)):
+                dict(temp=float("inf")), dict(temp=float("nan")), dict(red=3), dict(loss=None), dict(stats=None), dict(out=None), dict(cnt=None)):
         assert lib.axs6_distill_fwd(*(fwd | bad).values(), None) == ARG, bad
     assert lib.axs6_distill_fwd(*(fwd | dict(slots=1025)).values(), None) == UNSUPPORTED
     assert lib.axs6_distill_fwd(*(fwd | dict(stats=20)).values(), None) == ALIGN

@@ -121,3 +121,30 @@ def test_distillation_step_of_the_pipeline():
     assert all(not torch.equal(a, b) for a, b, n in zip(before, model.parameters(), (n for n, _ in model.named_parameters())) if "bias" not in n)
     again = pipe.distillation_step(batch, lambda b: (top, index))
     assert again["step"] == 2
+
+
+@pytest.mark.parametrize("D", [32, 33])
+def test_results_can_be_changed_in_place_and_saved_tensors_are_checked(D):
+    """The loss and rotated heads are tensors of their own: in-place changes behind them are differentiated.  Attention's backward pass needs
+    its output, and operands are saved: a change of those is reported."""
+    x = torch.randn(1, 2, 5, D, device="cuda").bfloat16().requires_grad_()
+    o = unified.axs_attention_unified(x, x, x)
+    o *= 2
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    z = torch.randn(4, 9, device="cuda", requires_grad=True)
+    top, index = torch.randn(4, 9, device="cuda").topk(3, -1)
+    for reduction in ("mean", "sum", "none"):
+        loss = unified.axs_distillation_unified(z, top, index, reduction=reduction)
+        want, = torch.autograd.grad(loss.sum(), z, retain_graph=True)
+        loss /= 4
+        got, = torch.autograd.grad(loss.sum(), z)
+        assert torch.equal(got, want / 4)
+    y, _ = unified.axs_rotary_unified(x.detach().requires_grad_()[..., :32], None, torch.arange(5, device="cuda"), unified.rotary_frequencies(32))
+    y += 1
+    y.sum().backward()
+    top2 = top.clone()
+    loss = unified.axs_distillation_unified(z, top2, index)
+    top2.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
