@@ -31,10 +31,6 @@ struct Params {
 };
 
 __device__ __forceinline__ float ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-__device__ __forceinline__ float to_f(float v) { return v; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_f(float v, float &o) { o = v; }
-__device__ __forceinline__ void from_f(float v, __nv_bfloat16 &o) { o = __float2bfloat16_rn(v); }
 
 __device__ __forceinline__ int keys_of(const Params &p, int b)
 {
@@ -78,6 +74,9 @@ __device__ __forceinline__ float masked_score(const Params &p, float x, int b, i
                                                : __bfloat162float(static_cast<const __nv_bfloat16 *>(p.mask)[at]);
     return m == -CUDART_INF_F ? m : x + m;
 }
+
+// The same with what masked_score gave for a score of 0: the mask's value, 0 where a truth value keeps the pair.
+__device__ __forceinline__ float under_mask(float x, float m) { return m == -CUDART_INF_F ? m : x + m; }
 
 // Implemented by the translation units of the kernels.
 int fwd_fp32(const Params &p, cudaStream_t st);

@@ -4,10 +4,10 @@
 // Forward, for 64 queries of one head: keys pass by in tiles of 64, x = scale Q K^T (+ mask), running maximum m and sum l of
 // exp(x - m), O rescaled whenever m grows.  Backward with P = exp(x - m) / l recomputed per tile:
 //     dV = P^T dO    dP = dO V^T    dS = P (dP - delta), delta = rowsum(dO O)    dQ = scale dS K    dK = scale dS^T Q
-// in two kernels: one per 64 queries for dQ, one per 64 keys for dK and dV, which also walks the query heads that share the key
+// in two kinds of CTAs: one per 64 queries for dQ, one per 64 keys for dK and dV, which also walks the query heads that share the key
 // head; so every output has one writer and a fixed order of summation, without atomics.
 //
-// Bound: fp32 FMA pipe (4 D flops a pair forward; 6 D and 8 D in the two backward kernels, which both recompute S and dP).  256 threads
+// Bound: fp32 FMA pipe (4 D flops a pair forward; 6 D and 8 D in the two halves of the backward pass, which both recompute S and dP).  256 threads
 // as 16 x 16; each owns 4 x 4 scores and 4 x D/16 outputs, operands in shared memory with rows padded by 16 bytes (a quarter warp's
 // 16-byte reads of eight rows then fall into different banks): 12 wavefronts of shared memory for 64 FMA instructions.
 #include "attn_common.cuh"
@@ -19,11 +19,11 @@ constexpr int kTile = 64, kThreads = 256;
 constexpr int kPStride = kTile + 4;
 
 // rows [r0, r0 + 64) of a (token, value) matrix into shared memory, zeros outside [0, limit) and behind the head's size
-template <typename T, int DP>
-__device__ __forceinline__ void load_tile(float *dst, const T *src, long long stride, int r0, int limit, int d, bool vec)
+template <int DP>
+__device__ __forceinline__ void load_tile(float *dst, const float *src, long long stride, int r0, int limit, int d, bool vec)
 {
     constexpr int S = DP + 4;
-    if (vec && sizeof(T) == 4) {
+    if (vec) {
         for (int i = threadIdx.x; i < kTile * (DP / 4); i += kThreads) {
             const int r = i / (DP / 4), c = (i - r * (DP / 4)) * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -33,7 +33,7 @@ __device__ __forceinline__ void load_tile(float *dst, const T *src, long long st
     } else {
         for (int i = threadIdx.x; i < kTile * DP; i += kThreads) {
             const int r = i / DP, c = i - r * DP;
-            dst[r * S + c] = (r0 + r < limit && c < d) ? to_f(src[(r0 + r) * stride + c]) : 0.0f;
+            dst[r * S + c] = (r0 + r < limit && c < d) ? src[(r0 + r) * stride + c] : 0.0f;
         }
     }
 }
@@ -87,8 +87,8 @@ __device__ __forceinline__ void rows_by_cols(const float *P, const float *B, int
             }
     }
 }
-template <typename T, int DP>
-__device__ __forceinline__ void store_rows(T *dst, long long stride, int r0, int limit, int d, int ty, int tx, const float acc[4][DP / 16], const float f[4])
+template <int DP>
+__device__ __forceinline__ void store_rows(float *dst, long long stride, int r0, int limit, int d, int ty, int tx, const float acc[4][DP / 16], const float f[4])
 {
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -97,9 +97,27 @@ __device__ __forceinline__ void store_rows(T *dst, long long stride, int r0, int
 #pragma unroll
         for (int e = 0; e < DP / 16; ++e) {
             const int c = 64 * (e / 4) + tx * 4 + e % 4;
-            if (c < d) from_f(acc[a][e] * f[a], dst[r * stride + c]);
+            if (c < d) dst[r * stride + c] = acc[a][e] * f[a];
         }
     }
+}
+
+// Whether every pair of 64 queries from i0 and 64 keys from j0 is visible but for a mask tensor.
+__device__ __forceinline__ bool whole_tile(const Params &p, int i0, int j0, int keys)
+{
+    return i0 + kTile <= p.q_len && j0 + kTile <= keys && (!p.causal || j0 + kTile - 1 <= i0 + p.offset) &&
+           (!p.window || j0 > i0 + kTile - 1 + p.offset - p.window);
+}
+// The mask's values for pairs (i0 + di(a), j0 + dj(c)), fetched before the products that they are added to; -inf hides a pair.
+template <typename I, typename J> __device__ __forceinline__ void fetch_mask(const Params &p, int b, int h, float mk[4][4], I query, J key, int keys)
+{
+#pragma unroll
+    for (int a = 0; a < 4; ++a)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const int i = query(a, c), j = key(a, c);
+            mk[a][c] = i < p.q_len && j < keys ? masked_score(p, 0.0f, b, h, i, j) : 0.0f;
+        }
 }
 
 __device__ __forceinline__ bool vec_ok(const View &v, int d)
@@ -107,8 +125,8 @@ __device__ __forceinline__ bool vec_ok(const View &v, int d)
     return ((reinterpret_cast<uintptr_t>(v.p) & 15u) | ((v.b | v.h | v.t | d) & 3)) == 0;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const Params p)
+template <int DP, bool kMask>
+__global__ void __launch_bounds__(kThreads, 2) simt_fwd_kernel(const Params p)
 {
     extern __shared__ __align__(16) float sm[];
     constexpr int S = DP + 4;
@@ -117,10 +135,10 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const Params p)
     const int bh = blockIdx.x % (p.batch * p.q_heads), h = bh % p.q_heads, b = bh / p.q_heads, kh = h / p.group;
     const int i0 = (int)((gridDim.x - 1 - blockIdx.x) / (p.batch * p.q_heads)) * kTile;      // the longest rows of a causal call first
     const int keys = keys_of(p, b);
-    const T *q = static_cast<const T *>(p.q.p) + b * p.q.b + h * p.q.h, *k = static_cast<const T *>(p.k.p) + b * p.k.b + kh * p.k.h,
-            *v = static_cast<const T *>(p.v.p) + b * p.v.b + kh * p.v.h;
+    const float *q = static_cast<const float *>(p.q.p) + b * p.q.b + h * p.q.h, *k = static_cast<const float *>(p.k.p) + b * p.k.b + kh * p.k.h,
+            *v = static_cast<const float *>(p.v.p) + b * p.v.b + kh * p.v.h;
     const bool qv = vec_ok(p.q, p.head_size), kv = vec_ok(p.k, p.head_size), vv = vec_ok(p.v, p.head_size);
-    load_tile<T, DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, qv);
+    load_tile<DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, qv);
     float m[4], l[4], acc[4][DP / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -132,8 +150,11 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const Params p)
     const int end = end_key(p, i1, keys);
     for (int j0 = first_key(p, i0) / kTile * kTile; j0 < end; j0 += kTile) {
         __syncthreads();
-        load_tile<T, DP>(Ks, k, p.k.t, j0, keys, p.head_size, kv);
-        load_tile<T, DP>(Vs, v, p.v.t, j0, keys, p.head_size, vv);
+        load_tile<DP>(Ks, k, p.k.t, j0, keys, p.head_size, kv);
+        load_tile<DP>(Vs, v, p.v.t, j0, keys, p.head_size, vv);
+        float mk[4][4];
+        if (kMask) fetch_mask(p, b, h, mk, [&](int a, int) { return i0 + ty * 4 + a; }, [&](int, int c) { return j0 + tx + 16 * c; }, keys);
+        const bool whole = whole_tile(p, i0, j0, keys);
         __syncthreads();
         float s[4][4];
         rows_by_rows<DP>(Qs, Ks, ty, tx, s);
@@ -144,7 +165,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const Params p)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int j = j0 + tx + 16 * c;
-                s[a][c] = sees(p, i, j, keys) ? masked_score(p, s[a][c] * p.scale, b, h, i, j) : -CUDART_INF_F;
+                s[a][c] = whole || sees(p, i, j, keys) ? (kMask ? under_mask(s[a][c] * p.scale, mk[a][c]) : s[a][c] * p.scale) : -CUDART_INF_F;
                 top = fmaxf(top, s[a][c]);
             }
             for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
@@ -178,40 +199,37 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(const Params p)
             if (p.lse) p.lse[at] = l[a] == 0.0f ? -CUDART_INF_F : m[a] + log2f(l[a]) * kLn2;
         }
     }
-    store_rows<T, DP>(static_cast<T *>(p.out) + b * p.out_b + h * p.out_h, p.out_t, i0, p.q_len, p.head_size, ty, tx, acc, inv);
+    store_rows<DP>(static_cast<float *>(p.out) + b * p.out_b + h * p.out_h, p.out_t, i0, p.q_len, p.head_size, ty, tx, acc, inv);
 }
 
 // delta = rowsum(dO * O): one warp a row.
-template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const Params p)
 {
     const long long rows = (long long)p.batch * p.q_heads * p.q_len;
     const long long row = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (row >= rows) return;
     const int i = (int)(row % p.q_len), h = (int)(row / p.q_len % p.q_heads), b = (int)(row / p.q_len / p.q_heads);
-    const T *o = static_cast<const T *>(p.o.p) + b * p.o.b + h * p.o.h + i * p.o.t;
-    const T *g = static_cast<const T *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h + i * p.d_o.t;
+    const float *o = static_cast<const float *>(p.o.p) + b * p.o.b + h * p.o.h + i * p.o.t;
+    const float *g = static_cast<const float *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h + i * p.d_o.t;
     float s = 0.0f;
-    for (int c = threadIdx.x & 31; c < p.head_size; c += 32) s = fmaf(to_f(o[c]), to_f(g[c]), s);
+    for (int c = threadIdx.x & 31; c < p.head_size; c += 32) s = fmaf(o[c], g[c], s);
     for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(~0u, s, x);
     if ((threadIdx.x & 31) == 0) p.delta[row] = s;
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_dq_kernel(const Params p)
+template <int DP, bool kMask> __device__ __forceinline__ void dq_body(const Params &p, float *sm, uint32_t block, uint32_t blocks)
 {
-    extern __shared__ __align__(16) float sm[];
     constexpr int S = DP + 4;
     float *Qs = sm, *Gs = Qs + kTile * S, *Ks = Gs + kTile * S, *Vs = Ks + kTile * S, *Ds = Vs + kTile * S;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int bh = blockIdx.x % (p.batch * p.q_heads), h = bh % p.q_heads, b = bh / p.q_heads, kh = h / p.group;
-    const int i0 = (int)((gridDim.x - 1 - blockIdx.x) / (p.batch * p.q_heads)) * kTile;
+    const int bh = block % (p.batch * p.q_heads), h = bh % p.q_heads, b = bh / p.q_heads, kh = h / p.group;
+    const int i0 = (int)((blocks - 1 - block) / (p.batch * p.q_heads)) * kTile;
     const int keys = keys_of(p, b);
-    const T *q = static_cast<const T *>(p.q.p) + b * p.q.b + h * p.q.h, *k = static_cast<const T *>(p.k.p) + b * p.k.b + kh * p.k.h,
-            *v = static_cast<const T *>(p.v.p) + b * p.v.b + kh * p.v.h, *g = static_cast<const T *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
+    const float *q = static_cast<const float *>(p.q.p) + b * p.q.b + h * p.q.h, *k = static_cast<const float *>(p.k.p) + b * p.k.b + kh * p.k.h,
+            *v = static_cast<const float *>(p.v.p) + b * p.v.b + kh * p.v.h, *g = static_cast<const float *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
     const bool kv = vec_ok(p.k, p.head_size), vv = vec_ok(p.v, p.head_size);
-    load_tile<T, DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, vec_ok(p.q, p.head_size));
-    load_tile<T, DP>(Gs, g, p.d_o.t, i0, p.q_len, p.head_size, vec_ok(p.d_o, p.head_size));
+    load_tile<DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, vec_ok(p.q, p.head_size));
+    load_tile<DP>(Gs, g, p.d_o.t, i0, p.q_len, p.head_size, vec_ok(p.d_o, p.head_size));
     float m[4], inv[4], delta[4], acc[4][DP / 16];
 #pragma unroll
     for (int a = 0; a < 4; ++a) {
@@ -228,10 +246,12 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(const Params p)
     const int end = end_key(p, i1, keys);
     for (int j0 = first_key(p, i0) / kTile * kTile; j0 < end; j0 += kTile) {
         __syncthreads();
-        load_tile<T, DP>(Ks, k, p.k.t, j0, keys, p.head_size, kv);
-        load_tile<T, DP>(Vs, v, p.v.t, j0, keys, p.head_size, vv);
+        load_tile<DP>(Ks, k, p.k.t, j0, keys, p.head_size, kv);
+        load_tile<DP>(Vs, v, p.v.t, j0, keys, p.head_size, vv);
         __syncthreads();
-        float s[4][4], d[4][4];
+        float s[4][4], d[4][4], mk[4][4];
+        if (kMask) fetch_mask(p, b, h, mk, [&](int a, int) { return i0 + ty * 4 + a; }, [&](int, int c) { return j0 + tx + 16 * c; }, keys);
+        const bool whole = whole_tile(p, i0, j0, keys);
         rows_by_rows<DP>(Qs, Ks, ty, tx, s);
         rows_by_rows<DP>(Gs, Vs, ty, tx, d);
 #pragma unroll
@@ -239,30 +259,28 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(const Params p)
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 const int i = i0 + ty * 4 + a, j = j0 + tx + 16 * c;
-                const float x = sees(p, i, j, keys) ? masked_score(p, s[a][c] * p.scale, b, h, i, j) : -CUDART_INF_F;
+                const float x = whole || sees(p, i, j, keys) ? (kMask ? under_mask(s[a][c] * p.scale, mk[a][c]) : s[a][c] * p.scale) : -CUDART_INF_F;
                 Ds[(ty * 4 + a) * kPStride + tx + 16 * c] = x == -CUDART_INF_F ? 0.0f : ex2((x - m[a]) * kLog2e) * inv[a] * (d[a][c] - delta[a]);
             }
         __syncwarp();
         rows_by_cols<DP>(Ds, Ks, ty, tx, acc);
     }
     const float f[4] = {p.scale, p.scale, p.scale, p.scale};
-    store_rows<T, DP>(static_cast<T *>(p.dq) + b * p.dq_b + h * p.dq_h, p.dq_t, i0, p.q_len, p.head_size, ty, tx, acc, f);
+    store_rows<DP>(static_cast<float *>(p.dq) + b * p.dq_b + h * p.dq_h, p.dq_t, i0, p.q_len, p.head_size, ty, tx, acc, f);
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads) simt_dkv_kernel(const Params p)
+template <int DP, bool kMask> __device__ __forceinline__ void dkv_body(const Params &p, float *sm, uint32_t block)
 {
-    extern __shared__ __align__(16) float sm[];
     constexpr int S = DP + 4;
     float *Ks = sm, *Vs = Ks + kTile * S, *Qs = Vs + kTile * S, *Gs = Qs + kTile * S, *Ps = Gs + kTile * S, *Ds = Ps + kTile * kPStride;
     float *Ms = Ds + kTile * kPStride, *Is = Ms + kTile, *Es = Is + kTile;
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int bh = blockIdx.x % (p.batch * p.k_heads), kh = bh % p.k_heads, b = bh / p.k_heads;
-    const int j0 = (int)(blockIdx.x / (p.batch * p.k_heads)) * kTile;
+    const int bh = block % (p.batch * p.k_heads), kh = bh % p.k_heads, b = bh / p.k_heads;
+    const int j0 = (int)(block / (p.batch * p.k_heads)) * kTile;
     const int keys = keys_of(p, b);
-    const T *k = static_cast<const T *>(p.k.p) + b * p.k.b + kh * p.k.h, *v = static_cast<const T *>(p.v.p) + b * p.v.b + kh * p.v.h;
-    load_tile<T, DP>(Ks, k, p.k.t, j0, keys, p.head_size, vec_ok(p.k, p.head_size));
-    load_tile<T, DP>(Vs, v, p.v.t, j0, keys, p.head_size, vec_ok(p.v, p.head_size));
+    const float *k = static_cast<const float *>(p.k.p) + b * p.k.b + kh * p.k.h, *v = static_cast<const float *>(p.v.p) + b * p.v.b + kh * p.v.h;
+    load_tile<DP>(Ks, k, p.k.t, j0, keys, p.head_size, vec_ok(p.k, p.head_size));
+    load_tile<DP>(Vs, v, p.v.t, j0, keys, p.head_size, vec_ok(p.v, p.head_size));
     const bool qv = vec_ok(p.q, p.head_size), gv = vec_ok(p.d_o, p.head_size);
     float ak[4][DP / 16], av[4][DP / 16];
 #pragma unroll
@@ -272,11 +290,11 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(const Params p)
     const int j1 = j0 + kTile < keys ? j0 + kTile : keys;
     const int end = j0 < keys ? end_query(p, j1) : 0;
     for (int h = kh * p.group; h < (kh + 1) * p.group; ++h) {
-        const T *q = static_cast<const T *>(p.q.p) + b * p.q.b + h * p.q.h, *g = static_cast<const T *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
+        const float *q = static_cast<const float *>(p.q.p) + b * p.q.b + h * p.q.h, *g = static_cast<const float *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
         for (int i0 = first_query(p, j0) / kTile * kTile; i0 < end; i0 += kTile) {
             __syncthreads();
-            load_tile<T, DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, qv);
-            load_tile<T, DP>(Gs, g, p.d_o.t, i0, p.q_len, p.head_size, gv);
+            load_tile<DP>(Qs, q, p.q.t, i0, p.q_len, p.head_size, qv);
+            load_tile<DP>(Gs, g, p.d_o.t, i0, p.q_len, p.head_size, gv);
             if (threadIdx.x < kTile) {
                 const int i = i0 + threadIdx.x;
                 const long long at = ((long long)b * p.q_heads + h) * p.q_len + i;
@@ -286,7 +304,9 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(const Params p)
                 Es[threadIdx.x] = i < p.q_len ? p.delta[at] : 0.0f;
             }
             __syncthreads();
-            float s[4][4], d[4][4];
+            float s[4][4], d[4][4], mk[4][4];
+            if (kMask) fetch_mask(p, b, h, mk, [&](int, int c) { return i0 + tx + 16 * c; }, [&](int a, int) { return j0 + ty * 4 + a; }, keys);
+            const bool whole = whole_tile(p, i0, j0, keys);
             rows_by_rows<DP>(Ks, Qs, ty, tx, s);
             rows_by_rows<DP>(Vs, Gs, ty, tx, d);
 #pragma unroll
@@ -294,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(const Params p)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     const int n = tx + 16 * c, i = i0 + n, j = j0 + ty * 4 + a;
-                    const float x = sees(p, i, j, keys) ? masked_score(p, s[a][c] * p.scale, b, h, i, j) : -CUDART_INF_F;
+                    const float x = whole || sees(p, i, j, keys) ? (kMask ? under_mask(s[a][c] * p.scale, mk[a][c]) : s[a][c] * p.scale) : -CUDART_INF_F;
                     const float w = x == -CUDART_INF_F ? 0.0f : ex2((x - Ms[n]) * kLog2e) * Is[n];
                     Ps[(ty * 4 + a) * kPStride + n] = w;
                     Ds[(ty * 4 + a) * kPStride + n] = w == 0.0f ? 0.0f : w * (d[a][c] - Es[n]);
@@ -305,45 +325,49 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(const Params p)
         }
     }
     const float fk[4] = {p.scale, p.scale, p.scale, p.scale}, fv[4] = {1.f, 1.f, 1.f, 1.f};
-    store_rows<T, DP>(static_cast<T *>(p.dk) + b * p.dk_b + kh * p.dk_h, p.dk_t, j0, p.k_len, p.head_size, ty, tx, ak, fk);
-    store_rows<T, DP>(static_cast<T *>(p.dv) + b * p.dv_b + kh * p.dv_h, p.dv_t, j0, p.k_len, p.head_size, ty, tx, av, fv);
+    store_rows<DP>(static_cast<float *>(p.dk) + b * p.dk_b + kh * p.dk_h, p.dk_t, j0, p.k_len, p.head_size, ty, tx, ak, fk);
+    store_rows<DP>(static_cast<float *>(p.dv) + b * p.dv_b + kh * p.dv_h, p.dv_t, j0, p.k_len, p.head_size, ty, tx, av, fv);
 }
 
-template <typename K>
-static int launch(K kernel, unsigned grid, int smem, const Params &p, cudaStream_t st)
+// The CTAs of both halves of the backward pass in one launch, those of dK and dV, which do more, first: small calls have no second tail.
+template <int DP, bool kMask> __global__ void __launch_bounds__(kThreads, DP == 64 ? 2 : 1) simt_bwd_kernel(const Params p, const uint32_t key_blocks)
 {
+    extern __shared__ __align__(16) float sm[];
+    if (blockIdx.x < key_blocks) dkv_body<DP, kMask>(p, sm, blockIdx.x);
+    else dq_body<DP, kMask>(p, sm, blockIdx.x - key_blocks, gridDim.x - key_blocks);
+}
+
+template <int DP> static int fwd_t(const Params &p, cudaStream_t st)
+{
+    const auto kernel = p.mask_kind == kMaskNone ? &simt_fwd_kernel<DP, false> : &simt_fwd_kernel<DP, true>;
+    const int smem = (3 * kTile * (DP + 4) + kTile * kPStride) * 4;
     if (!ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), smem)) return AXS6_ERR_LAUNCH;
+    const unsigned grid = (unsigned)((p.q_len + kTile - 1) / kTile) * (unsigned)(p.batch * p.q_heads);
     kernel<<<grid, kThreads, smem, st>>>(p);
     count_launch();
     return check_launch();
 }
-
-template <typename T, int DP> static int fwd_t(const Params &p, cudaStream_t st)
-{
-    const unsigned grid = (unsigned)((p.q_len + kTile - 1) / kTile) * (unsigned)(p.batch * p.q_heads);
-    return launch(&simt_fwd_kernel<T, DP>, grid, (3 * kTile * (DP + 4) + kTile * kPStride) * 4, p, st);
-}
-template <typename T, int DP> static int bwd_t(const Params &p, cudaStream_t st)
+template <int DP> static int bwd_t(const Params &p, cudaStream_t st)
 {
     const long long rows = (long long)p.batch * p.q_heads * p.q_len;
     if (rows) {
-        delta_kernel<T><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
+        delta_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
         count_launch();
-        int rc = check_launch();
-        if (rc != AXS6_OK) return rc;
-        const unsigned grid = (unsigned)((p.q_len + kTile - 1) / kTile) * (unsigned)(p.batch * p.q_heads);
-        rc = launch(&simt_dq_kernel<T, DP>, grid, (4 * kTile * (DP + 4) + kTile * kPStride) * 4, p, st);
+        const int rc = check_launch();
         if (rc != AXS6_OK) return rc;
     }
-    if (p.k_len) {
-        const unsigned grid = (unsigned)((p.k_len + kTile - 1) / kTile) * (unsigned)(p.batch * p.k_heads);
-        return launch(&simt_dkv_kernel<T, DP>, grid, (4 * kTile * (DP + 4) + 2 * kTile * kPStride + 3 * kTile) * 4, p, st);
-    }
-    return AXS6_OK;
+    const auto kernel = p.mask_kind == kMaskNone ? &simt_bwd_kernel<DP, false> : &simt_bwd_kernel<DP, true>;
+    const int smem = (4 * kTile * (DP + 4) + 2 * kTile * kPStride + 3 * kTile) * 4;
+    if (!ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), smem)) return AXS6_ERR_LAUNCH;
+    const uint32_t key_blocks = (uint32_t)((p.k_len + kTile - 1) / kTile) * (uint32_t)(p.batch * p.k_heads);
+    const uint32_t query_blocks = (uint32_t)((p.q_len + kTile - 1) / kTile) * (uint32_t)(p.batch * p.q_heads);
+    kernel<<<key_blocks + query_blocks, kThreads, smem, st>>>(p, key_blocks);
+    count_launch();
+    return check_launch();
 }
 
-int fwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? fwd_t<float, 64>(p, st) : fwd_t<float, 128>(p, st); }
-int bwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? bwd_t<float, 64>(p, st) : bwd_t<float, 128>(p, st); }
+int fwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? fwd_t<64>(p, st) : fwd_t<128>(p, st); }
+int bwd_fp32(const Params &p, cudaStream_t st) { return p.head_size <= 64 ? bwd_t<64>(p, st) : bwd_t<128>(p, st); }
 
 }  // namespace attn
 }  // namespace axs6
