@@ -39,8 +39,10 @@ template <int DP, bool kMask> static int fwd_launch(const Params &p, const CUten
 
 // Whether the few-queries kernel takes a call, and how the keys are cut.  It does when the stacked rows of a key head fit one tile, so that
 // a key tile is read once instead of once a query head, and when the other kernel's CTAs of 256 queries would leave half of the SMs idle.  Chunks:
-// about kFewPerSm CTAs an SM (two are resident; more even out different lengths), whole key tiles each.
-constexpr int kFewPerSm = 4;
+// about as many CTAs as are resident, whole key tiles each.  Twice as many even out batch entries of different lengths a little (16 entries of
+// 1 to 8 Ki keys, 8 key heads of 128: 70 against 73 us) and cost elsewhere, in prologues and in the join (1 entry of 64 Ki keys, 8 heads of 64:
+// 51 against 39 us).
+constexpr int kFewPerSm = 2;
 
 struct Plan { bool few; Few f; int64_t rows; };
 
