@@ -135,6 +135,10 @@ inline EncodeTiledFn encode_fn()
             qres == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<EncodeTiledFn>(ptr);
     });
+    // The encoder is a driver call and wants a current context.  A thread that has made no runtime call of its own yet (torch's backward
+    // thread) may have none: choosing the device that is current anyway binds its primary context, also during a stream capture.
+    int dev = -1;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaSetDevice(dev) != cudaSuccess) return nullptr;
     return fn;
 }
 

@@ -148,3 +148,27 @@ def test_results_can_be_changed_in_place_and_saved_tensors_are_checked(D):
     top2.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_backward_is_the_first_work_of_its_thread(dtype):
+    """A program whose backward thread has not used the device before attention's backward pass: the thread has no context of its own yet."""
+    import os
+    import subprocess
+    import sys
+    code = f"""
+import torch
+from torch.profiler import ProfilerActivity, profile
+from axs6_b200 import unified
+q, k, v, g = (torch.randn(1, 2, 64, 64, device="cuda").to(torch.{dtype}) for _ in range(4))
+leaves = [t.requires_grad_() for t in (q, k, v)]
+o = unified.axs_attention_unified(*leaves, causal=True)
+torch.cuda.synchronize()
+with profile(activities=[ProfilerActivity.CUDA]):
+    grads = torch.autograd.grad(o, leaves, g)
+    torch.cuda.synchronize()
+assert all(bool(t.isfinite().all()) for t in grads)
+print("done")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "done" in r.stdout, r.stderr[-1500:]
