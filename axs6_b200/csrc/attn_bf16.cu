@@ -98,7 +98,7 @@ template <int DP, bool kMask> static int bwd_launch(const Params &p, const CUten
     const RowData w = row_data(p);
     const long long rows = (long long)p.batch * p.q_heads * w.padded;
     if (rows) {
-        row_data_kernel<<<(unsigned)(rows / 64), 256, 0, st>>>(p, w, kMask);
+        row_data_kernel<DP / 8><<<(unsigned)(rows * (DP / 8) / 1024), 256, 0, st>>>(p, w, kMask);
         count_launch();
         const int rc = check_launch();
         if (rc != AXS6_OK) return rc;

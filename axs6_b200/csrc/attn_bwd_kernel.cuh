@@ -34,21 +34,26 @@ struct RowData {
     int padded;         // rows of a head
 };
 
-// 16 threads a row, 8 values each, four rows a thread
-__global__ void __launch_bounds__(256) row_data_kernel(const Params p, const RowData w, int mask)
+// kLanes threads a row, 8 values each, four rows a thread
+template <int kLanes> __global__ void __launch_bounds__(256) row_data_kernel(const Params p, const RowData w, int mask)
 {
-    const uint32_t tiles = (uint32_t)w.padded / 64u;                       // a CTA has 64 rows of one head
+    constexpr int kStep = 256 / kLanes, kCtaRows = 4 * kStep;              // 64 or 128 rows of one head
+    const uint32_t tiles = (uint32_t)(w.padded / kCtaRows);
     const uint32_t bh = blockIdx.x / tiles, h = bh % (uint32_t)p.q_heads, b = bh / (uint32_t)p.q_heads;
-    const int first = (int)(blockIdx.x - bh * tiles) * 64 + (int)(threadIdx.x >> 4), part = threadIdx.x & 15, c = part * 8;
+    const int first = (int)(blockIdx.x - bh * tiles) * kCtaRows + (int)threadIdx.x / kLanes, part = threadIdx.x % kLanes, c = part * 8;
     const __nv_bfloat16 *o = static_cast<const __nv_bfloat16 *>(p.o.p) + b * p.o.b + h * p.o.h;
     const __nv_bfloat16 *g = static_cast<const __nv_bfloat16 *>(p.d_o.p) + b * p.d_o.b + h * p.d_o.h;
     const __nv_bfloat16 *low = p.o_low ? static_cast<const __nv_bfloat16 *>(p.o_low) + (o - static_cast<const __nv_bfloat16 *>(p.o.p)) : nullptr;
     const uint4 none = make_uint4(0u, 0u, 0u, 0u);
     const bool whole = c + 8 <= p.head_size;
     uint4 x[4], y[4], t[4];
+    float m[4], l[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        const int i = first + 16 * n;
+        const int i = first + kStep * n;
+        const long long src = (long long)bh * p.q_len + i;
+        m[n] = i < p.q_len ? p.row_max[src] : 0.0f;
+        l[n] = i < p.q_len ? p.row_sum[src] : 0.0f;
         const bool here = whole && i < p.q_len;
         x[n] = here ? *reinterpret_cast<const uint4 *>(o + i * p.o.t + c) : none;
         y[n] = here ? *reinterpret_cast<const uint4 *>(g + i * p.d_o.t + c) : none;
@@ -56,7 +61,7 @@ __global__ void __launch_bounds__(256) row_data_kernel(const Params p, const Row
     }
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
-        const int i = first + 16 * n;
+        const int i = first + kStep * n;
         const uint32_t xs[4] = {x[n].x, x[n].y, x[n].z, x[n].w}, ys[4] = {y[n].x, y[n].y, y[n].z, y[n].w}, ts[4] = {t[n].x, t[n].y, t[n].z, t[n].w};
         float s = 0.0f;
 #pragma unroll
@@ -67,14 +72,10 @@ __global__ void __launch_bounds__(256) row_data_kernel(const Params p, const Row
         if (!whole && i < p.q_len)
             for (int e = c; e < p.head_size; ++e)
                 s = fmaf(__bfloat162float(o[i * p.o.t + e]) + (low ? __bfloat162float(low[i * p.o.t + e]) : 0.0f), __bfloat162float(g[i * p.d_o.t + e]), s);
-        for (int z = 8; z; z >>= 1) s += __shfl_xor_sync(~0u, s, z);
+        for (int z = kLanes / 2; z; z >>= 1) s += __shfl_xor_sync(~0u, s, z);
         if (part == 0) {
             float shift = mask ? 0.0f : CUDART_INF_F, log_sum = CUDART_INF_F;
-            if (i < p.q_len) {
-                const long long src = (long long)bh * p.q_len + i;
-                const float m = p.row_max[src], l = p.row_sum[src];
-                if (l != 0.0f) { log_sum = log2f(l); shift = mask ? m : fmaf(m, kLog2e, log_sum); }
-            }
+            if (l[n] != 0.0f) { log_sum = log2f(l[n]); shift = mask ? m[n] : fmaf(m[n], kLog2e, log_sum); }
             const long long at = (long long)bh * w.padded + i;
             w.shift[at] = shift;
             if (mask) w.log_sum[at] = log_sum;
