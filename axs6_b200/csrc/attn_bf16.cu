@@ -116,9 +116,8 @@ template <int DP, bool kMask> static int bwd_launch(const Params &p, const CUten
         const auto kernel = &dq_kernel<DP, kMask>;
         if (!ensure_dynamic_smem(reinterpret_cast<const void *>(kernel), DqSmem<DP>::kBytes)) return AXS6_ERR_LAUNCH;
         const unsigned grid = (unsigned)(w.padded / kRows) * (unsigned)(p.batch * p.q_heads);
-        kernel<<<grid, kBwdThreads, DqSmem<DP>::kBytes, st>>>(mq, mk, mv, mg, p, w);
+        if (launch_overlapped(p.k_len > 0, kernel, grid, kBwdThreads, DqSmem<DP>::kBytes, st, mq, mk, mv, mg, p, w) != cudaSuccess) return AXS6_ERR_LAUNCH;
         count_launch();
-        return check_launch();
     }
     return AXS6_OK;
 }

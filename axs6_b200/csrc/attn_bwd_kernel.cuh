@@ -120,6 +120,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     volatile uint32_t *slot = reinterpret_cast<volatile uint32_t *>(gen + L::kBars + kSlot);
     int *status = &g_status;
 
+    pdl_launch_dependents();                                              // the dQ kernel's CTAs may take the SMs that this grid's last ones leave
     const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
     const int heads = p.batch * p.k_heads;
     const int bh = blockIdx.x % heads, kh = bh % p.k_heads, b = bh / p.k_heads;
@@ -571,6 +572,9 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
             }
         }
     }
+    // Launched beside the dK, dV kernel, whose results it does not need: what both read was complete when that one began.  Waiting for it here
+    // lets work behind this kernel rely on both.
+    pdl_wait();
     fence_before();
     __syncthreads();
     linger_if_failed();
