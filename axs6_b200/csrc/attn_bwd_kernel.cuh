@@ -14,6 +14,8 @@
 //
 // Bound: tensor cores.  An M = 128, K = 16 product takes 64 clocks for any N up to 128: per 128 x 128 tile dK and dV 2048 clocks at D = 128 and
 // 1536 at D = 64, dQ 1536 and 1024; exp2 takes 1024 in each.  (Two sets at D = 128 with S and dP for 64 queries at a time: 3072, and slower.)
+// Measured, both kernels and the row sums: D = 128, 32 / 8 heads, 8192 x 8192, causal: 1500 us, 916 TFLOP/s of the five products and 1280 of the
+// seven that run, 0.92 of what the power cap leaves a plain GEMM; D = 64, 64 heads, 4096 x 4096: 1162 us; 16 x 8 heads, 1024 x 1024, causal: 151 us.
 #pragma once
 #include "attn_tc.cuh"
 

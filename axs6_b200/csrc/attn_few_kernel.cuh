@@ -8,8 +8,10 @@
 //
 // Bound: HBM, keys and values once.  Two CTAs live on an SM (half of tensor memory, 97 KB of shared memory each), so that one's products and
 // softmax run under the other's loads, and up to 128 KB are in flight on an SM.  Scores are double-buffered in tensor memory: S(j + 1) is
-// issued before P(j) V, so that the softmax of one tile runs under the products of its neighbours.  Warps 0-3: softmax, one thread a row; warps without rows
-// idle (the lanes of P that they would fill hold anything: a row of A reaches only its own row of the product).  Warp 4: products.  Warp 5: loads.
+// issued before P(j) V, so that the softmax of one tile runs under the products of its
+// neighbours.  Warps 0-3: softmax, one thread a row; warps without rows idle (the lanes of P that they would fill hold anything: a row of A reaches only its own row of the product).  Warp 4: products.
+// Warp 5: loads.  Measured: 16 entries of 8192 keys, 32 / 8 heads of 128: 109 us, 4.9 TB/s (0.75 of a copy); with 1 to 8 Ki keys 73 us for 48 us of
+// bytes; the tensor cores, which multiply 128 rows where 4 are wanted, are 40 % busy.
 #pragma once
 #include "attn_tc.cuh"
 

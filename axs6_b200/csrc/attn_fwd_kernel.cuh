@@ -14,9 +14,12 @@
 //
 // Score tiles (tile 0 and tile 1 in turn) rotate through the tensor memory that two output tiles leave: 2 buffers at D = 128, 3 at D = 64.  The
 // scores of unit u + buffers are computed behind P V of unit u; tcgen05 instructions of one thread complete in order, so they may overwrite its P.
-// Tiles of 64 keys with twice the buffers were 10 % slower at D = 128: an N = 64 product reads 6 KB of shared memory for 32 clocks of work.
+// Tiles of 64 keys with twice the buffers were 10 % slower at D = 128: an M = 128, K = 16 product takes 64 clocks for any N up to 128.
 //
-// Bound: 4 D flops a pair on the tensor cores (8192 a clock: 1024 clocks a tile at D = 128) and one exp2 a pair (16 a clock: 1024 clocks).
+// Bound: tensor cores, 4 D flops a pair (1024 clocks a tile of 128 x 128 at D = 128, 768 at D = 64), and one exp2 a pair (16 a clock: 1024
+// clocks).  Measured: D = 128, 32 / 8 heads, 8192 x 8192: 900 us, 1222 TFLOP/s, where the power cap holds a plain bf16 GEMM to 1393; causal 477 us,
+// 1150; D = 64, 64 heads, 4096 x 4096: 375 us, 733 TFLOP/s, exp2 unit 72 % busy.  A CTA's start, end and the gap to the next one take 6 us, which
+// is what short sequences pay (16 x 8 heads, 1024 x 1024, causal: 50 us for 15 us of tiles).
 #pragma once
 #include "attn_tc.cuh"
 

@@ -14,6 +14,9 @@
 // forward kernel, which joins their maxima and sums through distributed shared memory): several CTAs an SM are in different phases,
 // so that the ends of rows hide under the others' loads.  16-byte pieces where the row is aligned, single values up to the first boundary and
 // behind the last.  Sums are fp32 per thread (a few hundred terms) and joined in a fixed order.
+//
+// Measured, 8192 x 32000 bf16, 64 slots: forward 101 us (5.2 TB/s; the exp2 unit is 68 % busy), backward 157-167 us (6.3 TB/s); 1000 x 100001 fp32: 70
+// and 150 us; 7 x 32000 bf16: 8.4 and 6.4 us.  Short rows (5000 values) pay 97 us a pass at 16384 rows for 25 us of bytes: the ends of a row.
 #include <cuda_bf16.h>
 #include <math_constants.h>
 
