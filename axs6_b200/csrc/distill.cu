@@ -123,10 +123,8 @@ __device__ __forceinline__ uint32_t cluster_address(const void *shared, uint32_t
     asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"((uint32_t)__cvta_generic_to_shared(shared)), "r"(rank));
     return a;
 }
-__device__ __forceinline__ void cluster_sync()
-{
-    asm volatile("barrier.cluster.arrive.aligned;\n barrier.cluster.wait.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;" ::: "memory"); }
 
 template <typename T, typename Tt>
 __global__ void __launch_bounds__(kThreads, 4) forward_kernel(const Params p)
@@ -167,6 +165,7 @@ __global__ void __launch_bounds__(kThreads, 4) forward_kernel(const Params p)
         if (seg == 0 && threadIdx.x == 0) { p.row_loss[row] = 0.0f; p.stats[row] = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
         return;
     }
+    if (p.segments > 1) cluster_arrive();                           // the segments' CTAs run: their shared memory may be written to
     float picked[kSlotRounds];
 #pragma unroll
     for (int x = 0; x < kSlotRounds; ++x) picked[x] = seg == 0 && mine[x] >= 0 ? to_f(z[mine[x]]) : 0.0f;
@@ -240,12 +239,16 @@ __global__ void __launch_bounds__(kThreads, 4) forward_kernel(const Params p)
         for (int o = kWarps / 2; o; o >>= 1) join(m, s, __shfl_xor_sync(~0u, m, o), __shfl_xor_sync(~0u, s, o), c);
     }
     if (p.segments > 1) {
+        __syncwarp();
+        cluster_wait();
         if (threadIdx.x == 0) {
             const uint32_t a = cluster_address(joined + 2 * seg, 0);
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a), "f"(m) : "memory");
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(a + 4u), "f"(s) : "memory");
         }
-        cluster_sync();
+        __syncwarp();
+        cluster_arrive();
+        cluster_wait();
         if (seg == 0 && threadIdx.x < 32) {
             m = -CUDART_INF_F; s = 0.0f;
             for (int x = 0; x < p.segments; ++x) join(m, s, joined[2 * x], joined[2 * x + 1], c);

@@ -7,6 +7,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -26,6 +27,7 @@ class _Attention(torch.autograd.Function):
         return o, lse
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o, *unused):
         q, k, v, o, low, stats, key_lengths, mask = ctx.saved_tensors
         dq, dk, dv = ops.attention_bwd(d_o, q, k, v, o, low, stats, key_lengths, mask, *ctx.call)

@@ -7,6 +7,7 @@ there).  ``axs_distillation_unified`` is the loss, ``AXSDistillationLoss`` the f
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -25,6 +26,7 @@ class _Distillation(torch.autograd.Function):
         return loss
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, upstream):
         z, t, index, stats, count = ctx.saved_tensors
         grad = ops.distill_bwd(z, t, index, stats, upstream, count, ctx.temperature)

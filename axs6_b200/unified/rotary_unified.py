@@ -9,6 +9,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -82,6 +83,7 @@ class _Rotary(torch.autograd.Function):
         return ops.rotary(q, k, positions, turns, gain, interleaved, False, who="axs_rotary_unified")
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         positions, turns = ctx.saved_tensors
         if dq is None and dk is None:

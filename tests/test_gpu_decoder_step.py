@@ -172,3 +172,15 @@ print("done")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))), capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "done" in r.stdout, r.stderr[-1500:]
+
+
+def test_second_derivatives_are_refused():
+    x = torch.randn(1, 1, 4, 8, device="cuda", requires_grad=True)
+    z, top, index = torch.randn(2, 6, device="cuda", requires_grad=True), torch.randn(2, 2, device="cuda"), torch.tensor([[0, 1], [2, 3]], device="cuda")
+    plan, pos = unified.rotary_frequencies(8), torch.arange(4, device="cuda")
+    for leaf, out in ((x, unified.axs_attention_unified(x, x, x).sum()), (x, unified.axs_rotary_unified(x, None, pos, plan)[0].pow(2).sum()),
+                      (z, unified.axs_distillation_unified(z, top, index))):
+        g, = torch.autograd.grad(out, leaf, create_graph=True)
+        # without a graph behind the gradient, or with one that says so, whichever the upstream gradient leads to
+        with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+            g.sum().backward()
