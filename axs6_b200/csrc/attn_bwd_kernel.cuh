@@ -186,12 +186,13 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
     } else if (warp == 16) {
         if (steps > 0) {
             const bool one = elect();
+            const int slices = (p.head_size + 15) / 16;
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kStage; };
             const auto scores = [&](int x) {                              // S^T = K Q^T
                 if (!wait_warp(q_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, 22, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tS(x), base, stage(x));
+                    product_rows<DP>(tS(x), base, stage(x), slices);
                     commit(s_full(x));
                 }
                 __syncwarp();
@@ -201,7 +202,7 @@ dkv_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 if (!wait_warp(g_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, 23, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tD, base + L::kTile, stage(x) + L::kTile);
+                    product_rows<DP>(tD, base + L::kTile, stage(x) + L::kTile, slices);
                     commit(d_full(x));
                 }
                 __syncwarp();
@@ -453,13 +454,14 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
     } else if (warp == 16) {
         if (steps > 0) {
             const bool one = elect();
+            const int slices = (p.head_size + 15) / 16;
             const auto kt = [&](int x) { return base + L::kRingK + (uint32_t)(x % L::kK) * L::kTile; };
             const auto vt = [&](int x) { return base + L::kRingV + (uint32_t)(x % L::kV) * L::kTile; };
             const auto scores = [&](int x) {                              // S = Q K^T
                 if (!wait_warp(k_full(x % L::kK), (uint32_t)(x / L::kK) & 1u, 24, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tS(x), base, kt(x));
+                    product_rows<DP>(tS(x), base, kt(x), slices);
                     commit(s_full(x));
                 }
                 __syncwarp();
@@ -469,7 +471,7 @@ dq_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUtens
                 if (!wait_warp(v_full(x % L::kV), (uint32_t)(x / L::kV) & 1u, 25, status)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tD, base + L::kTile, vt(x));
+                    product_rows<DP>(tD, base + L::kTile, vt(x), slices);
                     commit(d_full(x));
                     commit(v_empty(x % L::kV));
                 }

@@ -111,13 +111,14 @@ few_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUten
     } else if (warp == 4) {
         if (steps > 0) {
             const bool one = elect();
+            const int slices = (p.head_size + 15) / 16;
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kTile; };
             const auto full = [&](int x, int code) { return wait_warp(kv_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, code, status); };
             const auto scores = [&](int j) {
                 if (!full(2 * j, 4)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP, kKeys>(tmem + 64u * (j & 1), base, stage(2 * j));
+                    product_rows<DP, kKeys>(tmem + 64u * (j & 1), base, stage(2 * j), slices);
                     commit(s_full(j & 1));
                     commit(kv_empty((2 * j) % L::kStages));
                 }

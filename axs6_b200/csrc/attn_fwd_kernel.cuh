@@ -141,6 +141,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
         // ------------------------------------------------------------------ products
         if (steps > 0) {
             const bool one = elect();
+            const int slices = (p.head_size + 15) / 16;
             const auto stage = [&](int x) { return base + L::kRing + (uint32_t)(x % L::kStages) * L::kTile; };
             const auto full = [&](int x, int code) { return wait_warp(kv_full(x % L::kStages), (uint32_t)(x / L::kStages) & 1u, code, status); };
             const int units = n0 + n1, first = n0 > 0 ? 0 : 1;                    // tile 1 alone walks where tile 0 sees nothing
@@ -152,7 +153,7 @@ fwd_kernel(const __grid_constant__ CUtensorMap mq, const __grid_constant__ CUten
                 if (!full(2 * j, 3)) return false;
                 fence_after();
                 if (one) {
-                    product_rows<DP>(tS(u % kBufs), base + t * L::kTile, stage(2 * j));
+                    product_rows<DP>(tS(u % kBufs), base + t * L::kTile, stage(2 * j), slices);
                     commit(s_full(u % kBufs));
                     if (last_of_step(u)) commit(kv_empty((2 * j) % L::kStages));
                 }

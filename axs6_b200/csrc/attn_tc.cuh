@@ -87,14 +87,14 @@ __host__ __device__ constexpr uint32_t instr(int n, int b_mn)
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 }
 
-// D (128 x kTokens) = A B^T over the head's DP values, tiles at shared addresses `a` (128 rows) and `b` (kTokens rows), both K-major
-template <int DP, int kTokens = kRows> __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b)
+// D (128 x kTokens) = A B^T over the head's first 16 `slices` values (behind its size the tiles hold zeros), tiles at shared addresses `a` (128 rows) and `b` (kTokens rows), both K-major
+template <int DP, int kTokens = kRows> __device__ __forceinline__ void product_rows(uint32_t d, uint32_t a, uint32_t b, int slices)
 {
     const uint32_t al = desc_low(a, 0), bl = desc_low(b, 0);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
         const uint32_t box = (uint32_t)(k / 4), step = (uint32_t)(k % 4) * 2u;
-        mma_ss(d, al + box * (kBox >> 4) + step, bl + box * (kTokens * 128u >> 4) + step, instr(kTokens, 0), k != 0);
+        if (k < slices) mma_ss(d, al + box * (kBox >> 4) + step, bl + box * (kTokens * 128u >> 4) + step, instr(kTokens, 0), k != 0);
     }
 }
 // D (128 x DP) (+)= A B over kTokens tokens: A is 128 x kTokens bf16 in tensor memory (two values a column), B a tile, MN-major.  kGroup: A's
