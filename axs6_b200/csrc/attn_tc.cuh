@@ -17,9 +17,9 @@ namespace tc {
 using acp::smem_u32;
 
 constexpr int kRows = 128;                       // tokens of a tile
-constexpr int kKeys = 64;                        // keys of a tile of the forward kernels
+constexpr int kKeys = 64;                        // keys of a tile of the few-queries kernel
 constexpr uint32_t kBox = 128 * 128;             // bytes of a box
-constexpr uint32_t kWaitPolls = 1u << 20;        // of about a microsecond each, when a poll has to sleep
+constexpr uint32_t kWaitPolls = 1u << 20;        // a poll sleeps for as long as the hardware lets it; all of them about a second
 
 static __device__ int g_status;                  // 0, or the code of the first wait that gave up (one translation unit includes this)
 
